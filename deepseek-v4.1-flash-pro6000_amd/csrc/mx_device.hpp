@@ -6,6 +6,7 @@
 #include <stdint.h>
 #include "ds41_moe_gfx950.h"
 #include "ds41_accept_gfx950.h"
+#include "ds41_logits_gfx950.h"
 
 namespace ds41g {
 
@@ -25,8 +26,9 @@ constexpr int kMaxJobTokens = 8;   // rows per expert job (reference GemmJob: 1.
 constexpr int kWave = 64;
 
 // Kernel-visible status bits (ds41_status): a bounded wait that gave up, or a
-// job descriptor whose row count is outside 1..kMaxJobTokens.
-enum : uint32_t { kStatusReadyTimeout = 1u, kStatusBadJob = 2u, kStatusBadRoute = 4u };
+// job descriptor whose row count is outside 1..kMaxJobTokens, invalid routes, or a
+// row of logits whose mask allows nothing.
+enum : uint32_t { kStatusReadyTimeout = 1u, kStatusBadJob = 2u, kStatusBadRoute = 4u, kStatusEmptyMask = 8u };
 extern __device__ uint32_t ds41_status;
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }

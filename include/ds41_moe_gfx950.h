@@ -373,6 +373,23 @@ int ds41_dense_fp8(const void *a_fp8, const void *as_ue8m0, const void *w_fp8, c
 int ds41_dense_shared_act(const void *gate_bf16, const void *up_bf16, void *z_bf16, void *a_fp8,
                           void *as_ue8m0, int M, int K, void *stream);
 
+/* ---- bf16 dense product (the head and the model's bf16 projections) --------------- */
+/* y = act(x w^T + bias) + residual: x bf16 [M][K] (rows ldx apart), w bf16 [N][K] (ldw), bias F32 [N]
+ * (nullable), residual [M][N] (ldr) in y's type (nullable; may be y with ldr == ldy), y [M][N] (ldy) of type
+ * DS41_TYPE_F32 or DS41_TYPE_BF16 (ds41_logits_gfx950.h). Sums, bias, activation and residual are fp32; y is
+ * rounded once. No operand but residual may overlap y. M, N, K 1 .. 1,048,576, strides in elements, rows
+ * aligned to their element; rows of 16-byte multiples at 16-byte addresses take the fast paths. No counterpart
+ * in the reference's own kernels (its bf16 head and projections are library and generated code,
+ * components/fuse-head, components/dense/include/ds41/dense.h:28).
+ * workspace (nullable): ds41_dense_bf16_workspace_bytes(M, N, K) device bytes, 256-byte aligned, let a product
+ * of few output tiles be split over K (partial sums in a fixed order: the same bits every call). Without it,
+ * or with less, the product is not split; calls that share one must be ordered. */
+enum { DS41_ACT_NONE = 0, DS41_ACT_RELU = 1, DS41_ACT_SILU = 2, DS41_ACT_GELU = 3 /* exact, with erf */ };
+size_t ds41_dense_bf16_workspace_bytes(int M, int N, int K);
+int ds41_dense_bf16(const void *x_bf16, size_t ldx, const void *w_bf16, size_t ldw, const float *bias,
+                    const void *residual, size_t ldr, void *y, size_t ldy, int y_type, int M, int N, int K,
+                    int act, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- expert slot pool (LFU residency policy) and placement files ------------- */
 /* The reference's SlotPool (components/moe/include/ds41/store.hpp:80-157, store.cpp:15-196): a
  * CPU-only, deterministic assignment of experts to HBM slots. Expert ids are flattened layer by
@@ -618,7 +635,8 @@ int ds41_hbm_read_probe_ex(const void *buf, size_t bytes, void *sink, int blocks
 int ds41_e4m3_converter_check(unsigned long long *mismatches, void *stream);
 /* Reads and clears the kernels' status bits (synchronous): 1 a residency wait
  * gave up (the rows that needed those weights are written as NaN), 2 a job's
- * row count was outside 1..8, 4 invalid/duplicate routes. */
+ * row count was outside 1..8, 4 invalid/duplicate routes, 8 a row of logits whose
+ * mask allows nothing (ds41_logits_control). */
 int ds41_take_status(uint32_t *status);
 
 #ifdef __cplusplus
