@@ -432,31 +432,48 @@ def dense_shared_act(g, u, stream=None):
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}  # DS41_ACT_*
 
 
+def _dtypes():
+    """(float32, bfloat16, int32), with torch imported on first use; the checks below compare by identity, a call's
+    share of host time being as long as a small kernel."""
+    global _DTYPES
+    if _DTYPES is None:
+        import torch
+        _DTYPES = (torch.float32, torch.bfloat16, torch.int32)
+    return _DTYPES
+
+
+_DTYPES = None
+
+
 def _type(t):
     """DS41_TYPE_* of a tensor of logits, gradients or products."""
-    import torch
-    if t.dtype == torch.float32:
+    f32, bf16, _ = _dtypes()
+    d = t.dtype
+    if d is f32:
         return 0
-    if t.dtype == torch.bfloat16:
+    if d is bf16:
         return 1
-    raise ValueError(f"float32 or bfloat16, not {t.dtype}")
+    raise ValueError(f"float32 or bfloat16, not {d}")
 
 
 def _rows(t, what, dtype=None):
     """Row stride of a matrix whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (dtype is not None and t.dtype != dtype):
-        raise ValueError(f"{what}: a matrix with contiguous rows" + (f" of {dtype}" if dtype else "") +
-                         f", not {tuple(t.shape)} {t.dtype} with strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    st = t.stride()
+    if len(st) == 2 and (dtype is None or t.dtype is dtype):
+        n, cols = t.shape
+        if st[1] == 1 or cols <= 1:
+            return st[0] if n > 1 or st[0] > cols else cols
+    raise ValueError(f"{what}: a matrix with contiguous rows" + (f" of {dtype}" if dtype else "") +
+                     f", not {tuple(t.shape)} {t.dtype} with strides {st}")
 
 
 def _flat(t, what, dtype, n):
     """Address of a contiguous tensor of n elements (at least), or null."""
     if t is None:
         return None
-    if t.dtype != dtype or not t.is_contiguous() or t.numel() < n:
-        raise ValueError(f"{what}: {n} contiguous elements of {dtype}, not {tuple(t.shape)} {t.dtype}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.numel() >= n and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{what}: {n} contiguous elements of {dtype}, not {tuple(t.shape)} {t.dtype}")
 
 
 def dense_bf16_workspace_bytes(M, N, K):
@@ -466,21 +483,23 @@ def dense_bf16_workspace_bytes(M, N, K):
 def dense_bf16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=None, workspace=None, stream=None):
     """act(x w^T + bias) + residual, x bf16 [M][K], w bf16 [N][K], into out (or a new tensor of out_dtype,
     bfloat16 by default)."""
-    import torch
-    ldx, ldw = _rows(x, "x", torch.bfloat16), _rows(w, "w", torch.bfloat16)
-    (M, K), N = x.shape, w.shape[0]
-    if w.shape[1] != K:
-        raise ValueError(f"x has {K} columns, w {w.shape[1]}")
+    f32, bf16, _ = _dtypes()
+    ldx, ldw = _rows(x, "x", bf16), _rows(w, "w", bf16)
+    (M, K), (N, Kw) = x.shape, w.shape
+    if Kw != K:
+        raise ValueError(f"x has {K} columns, w {Kw}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=x.device)
-    if tuple(out.shape) != (M, N) or (residual is not None and tuple(residual.shape) != (M, N)):
-        raise ValueError(f"out and residual have shape {(M, N)}")
-    ldy = _rows(out, "out")
-    ldr = 0 if residual is None else _rows(residual, "residual", out.dtype)
-    check(lib().ds41_dense_bf16(x.data_ptr(), ldx, w.data_ptr(), ldw, _flat(bias, "bias", torch.float32, N), _p(residual), ldr,
-                                out.data_ptr(), ldy, _type(out), M, N, K, ACTS[act], _p(workspace),
-                                0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(stream)),
-          "ds41_dense_bf16")
+        out = x.new_empty((M, N), dtype=out_dtype or bf16)
+    elif out.shape != (M, N):
+        raise ValueError(f"out has shape {(M, N)}, not {tuple(out.shape)}")
+    ldr, res = 0, None
+    if residual is not None:
+        if residual.shape != (M, N):
+            raise ValueError(f"residual has shape {(M, N)}, not {tuple(residual.shape)}")
+        ldr, res = _rows(residual, "residual", out.dtype), residual.data_ptr()
+    ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+    check(lib().ds41_dense_bf16(x.data_ptr(), ldx, w.data_ptr(), ldw, _flat(bias, "bias", f32, N), res, ldr, out.data_ptr(),
+                                _rows(out, "out"), _type(out), M, N, K, ACTS[act], ws, size, _stream(stream)), "ds41_dense_bf16")
     return out
 
 
@@ -1173,38 +1192,34 @@ def token_counts(table_rows, vocab, device="cuda"):
 
 
 def _table(counts, seen, vocab):
-    import torch
-    rows = (counts if counts is not None else seen).shape[0]
-    return (_flat(counts, "counts", torch.int32, rows * vocab), _flat(seen, "seen", torch.int32, rows * ((vocab + 31) // 32)), rows)
+    rows, i32 = (counts if counts is not None else seen).shape[0], _dtypes()[2]
+    return _flat(counts, "counts", i32, rows * vocab), _flat(seen, "seen", i32, rows * ((vocab + 31) // 32)), rows
 
 
 def token_counts_clear(counts, seen, vocab, table_index=None, stream=None):
     """Empties every table row, or the ones in table_index."""
-    import torch
     c, s, rows = _table(counts, seen, vocab)
     n = rows if table_index is None else table_index.numel()
-    check(lib().ds41_token_counts_clear(c, s, rows, vocab, _flat(table_index, "table_index", torch.int32, n), n, _stream(stream)),
+    check(lib().ds41_token_counts_clear(c, s, rows, vocab, _flat(table_index, "table_index", _dtypes()[2], n), n, _stream(stream)),
           "ds41_token_counts_clear")
 
 
 def token_counts_add(counts, seen, vocab, tokens, offsets, table_index=None, generated=True, stream=None):
     """Sequence i adds tokens[offsets[i]:offsets[i + 1]] to table row table_index[i] (row i): marked, and counted
     where the answer generated them."""
-    import torch
     c, s, rows = _table(counts, seen, vocab)
     n = offsets.numel() - 1
-    check(lib().ds41_token_counts_add(c, s, rows, vocab, _flat(table_index, "table_index", torch.int32, n),
-                                      _flat(tokens, "tokens", torch.int32, 0), _flat(offsets, "offsets", torch.int32, 2), n,
+    check(lib().ds41_token_counts_add(c, s, rows, vocab, _flat(table_index, "table_index", _dtypes()[2], n),
+                                      _flat(tokens, "tokens", _dtypes()[2], 0), _flat(offsets, "offsets", _dtypes()[2], 2), n,
                                       tokens.numel(), int(generated), _stream(stream)), "ds41_token_counts_add")
 
 
 def token_counts_commit(counts, seen, vocab, results, n=1, table_index=None, stream=None):
     """Adds the tokens of n ds41_spark_result (a device tensor, as verify_logits writes it)."""
-    import torch
     c, s, rows = _table(counts, seen, vocab)
-    if results.numel() * results.element_size() < n * ctypes.sizeof(SparkResult) or not results.is_contiguous():
+    if results.nbytes < n * ctypes.sizeof(SparkResult) or not results.is_contiguous():
         raise ValueError(f"results: {n} contiguous ds41_spark_result")
-    check(lib().ds41_token_counts_commit(c, s, rows, vocab, _flat(table_index, "table_index", torch.int32, n), results.data_ptr(), n,
+    check(lib().ds41_token_counts_commit(c, s, rows, vocab, _flat(table_index, "table_index", _dtypes()[2], n), results.data_ptr(), n,
                                          _stream(stream)), "ds41_token_counts_commit")
 
 
@@ -1214,88 +1229,101 @@ LOWEST = -3.4028234663852886e38  # a masked value that the samplers take (they r
 def logits_control(logits, rows=1, counts=None, seen=None, table_index=None, drafts=None, penalties=None, bias_ids=None,
                    bias_values=None, bias_offsets=None, mask=None, mask_index=None, masked_value=LOWEST, out=None, stream=None):
     """Penalties, biases and grammar masks on fp32 logits [sequences * rows][vocab], in place unless out is given."""
-    import torch
-    out = logits if out is None else out
-    ld_in, ld_out = _rows(logits, "logits", torch.float32), _rows(out, "out", torch.float32)
+    f32, _, i32 = _dtypes()
     n, V = logits.shape
-    if rows < 1 or n % rows or tuple(out.shape) != (n, V):
+    ld_in = _rows(logits, "logits", f32)
+    if out is None:
+        out, ld_out = logits, ld_in
+    else:
+        ld_out = _rows(out, "out", f32)
+    if rows < 1 or n % rows or out.shape != (n, V):
         raise ValueError(f"{n} rows are not whole sequences of {rows}, or out is not {(n, V)}")
-    S, i32 = n // rows, torch.int32
+    S = n // rows
     c, s, table_rows = _table(counts, seen, V) if counts is not None or seen is not None else (None, None, 0)
-    total = 0 if bias_ids is None else bias_ids.numel()
+    d, draft_ld, total, mask_p, mask_ld, mask_rows = None, 0, 0, None, 0, 0
+    if drafts is not None:
+        draft_ld = drafts.shape[-1]
+        d = _flat(drafts, "drafts", i32, S * draft_ld)
+    if bias_ids is not None:
+        total = bias_ids.numel()
+    if mask is not None:
+        mask_p, mask_ld, mask_rows = mask.data_ptr(), _rows(mask, "mask", i32), mask.shape[0]
     check(lib().ds41_logits_control(
-        logits.data_ptr(), ld_in, out.data_ptr(), ld_out, S, rows, V, c, s, table_rows, _flat(table_index, "table_index", i32, S),
-        None if drafts is None else _flat(drafts, "drafts", i32, S * drafts.shape[-1]), 0 if drafts is None else drafts.shape[-1],
-        _flat(penalties, "penalties", torch.float32, 3 * S), _flat(bias_ids, "bias_ids", i32, 0),
-        _flat(bias_values, "bias_values", torch.float32, total), _flat(bias_offsets, "bias_offsets", i32, S + 1), total, _p(mask),
-        0 if mask is None else _rows(mask, "mask", i32), 0 if mask is None else mask.shape[0], _flat(mask_index, "mask_index", i32, n),
+        logits.data_ptr(), ld_in, out.data_ptr(), ld_out, S, rows, V, c, s, table_rows, _flat(table_index, "table_index", i32, S), d, draft_ld,
+        _flat(penalties, "penalties", f32, 3 * S), _flat(bias_ids, "bias_ids", i32, 0), _flat(bias_values, "bias_values", f32, total),
+        _flat(bias_offsets, "bias_offsets", i32, S + 1), total, mask_p, mask_ld, mask_rows, _flat(mask_index, "mask_index", i32, n),
         masked_value, _stream(stream)), "ds41_logits_control")
     return out
 
 
-def _workspace(t, need, device):
-    """(tensor, bytes) of a workspace, a new one where none is given (kept by torch's allocator for the stream)."""
-    import torch
+def _workspace(t, need, like, stream):
+    """(address, bytes, tensor) of a workspace, of a new one of need() bytes where none is given, whose memory torch's
+    allocator keeps for the stream that the call uses."""
     if t is None:
-        t = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
-    return t, t.numel() * t.element_size()
+        import torch
+        t = torch.empty(max(need(), 1), dtype=torch.uint8, device=like.device)
+        if stream is not None:
+            t.record_stream(stream)
+    return t.data_ptr(), t.nbytes, t
 
 
 def top_logits(logits, k, temperature=1.0, chosen=None, ids=None, values=None, lse=None, logprob=None, workspace=None, stream=None):
     """(ids [rows][k], values [rows][k], lse [rows], logprob [rows] or None without chosen) of fp32 or bf16 rows."""
-    import torch
-    ld, (n, V), dev, f32 = _rows(logits, "logits"), logits.shape, logits.device, torch.float32
-    ids = torch.empty((n, k), dtype=torch.int32, device=dev) if ids is None else ids
-    values = torch.empty((n, k), device=dev) if values is None else values
-    lse = torch.empty(n, device=dev) if lse is None else lse
-    if chosen is not None and logprob is None:
-        logprob = torch.empty(n, device=dev)
-    ws, size = _workspace(workspace, 0 if workspace is not None else lib().ds41_top_logits_workspace_bytes(n, V, k), dev)
-    check(lib().ds41_top_logits(logits.data_ptr(), _type(logits), ld, n, V, k, temperature, _flat(ids, "ids", torch.int32, n * k),
-                                _flat(values, "values", f32, n * k), _flat(lse, "lse", f32, n),
-                                _flat(chosen, "chosen", torch.int32, n), None if chosen is None else _flat(logprob, "logprob", f32, n),
-                                ws.data_ptr(), size, _stream(stream)), "ds41_top_logits")
+    f32, _, i32 = _dtypes()
+    ld, (n, V) = _rows(logits, "logits"), logits.shape
+    ids = logits.new_empty((n, k), dtype=i32) if ids is None else ids
+    values = logits.new_empty((n, k), dtype=f32) if values is None else values
+    lse = logits.new_empty(n, dtype=f32) if lse is None else lse
+    lp = None
+    if chosen is not None:
+        logprob = logits.new_empty(n, dtype=f32) if logprob is None else logprob
+        lp = _flat(logprob, "logprob", f32, n)
+    ws, size, keep = _workspace(workspace, lambda: lib().ds41_top_logits_workspace_bytes(n, V, k), logits, stream)
+    check(lib().ds41_top_logits(logits.data_ptr(), _type(logits), ld, n, V, k, temperature, _flat(ids, "ids", i32, n * k),
+                                _flat(values, "values", f32, n * k), _flat(lse, "lse", f32, n), _flat(chosen, "chosen", i32, n), lp,
+                                ws, size, _stream(stream)), "ds41_top_logits")
     return ids, values, lse, logprob if chosen is not None else None
 
 
 def _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature):
     """The arguments that the distillation calls share."""
-    import torch
-    ld, (n, V), k = _rows(logits, "logits"), logits.shape, teacher_ids.shape[-1]
-    return (logits.data_ptr(), _type(logits), ld, n, V, _flat(teacher_ids, "teacher_ids", torch.int32, n * k),
-            _flat(teacher_logits, "teacher_logits", torch.float32, n * k), k, _flat(teacher_lse, "teacher_lse", torch.float32, n),
-            temperature)
+    f32, _, i32 = _dtypes()
+    (n, V), k = logits.shape, teacher_ids.shape[-1]
+    return (logits.data_ptr(), _type(logits), _rows(logits, "logits"), n, V, _flat(teacher_ids, "teacher_ids", i32, n * k),
+            _flat(teacher_logits, "teacher_logits", f32, n * k), k, _flat(teacher_lse, "teacher_lse", f32, n), temperature)
+
+
+def _loss(logits, loss, stats, workspace, stream):
+    """loss, stats and workspace of a forward call, with their addresses."""
+    f32, (n, V) = _dtypes()[0], logits.shape
+    loss = logits.new_empty(n, dtype=f32) if loss is None else loss
+    stats = logits.new_empty((n, 2), dtype=f32) if stats is None else stats
+    ws = _workspace(workspace, lambda: lib().ds41_distill_workspace_bytes(n, V), logits, stream)
+    return loss, stats, _flat(loss, "loss", f32, n), _flat(stats, "stats", f32, 2 * n), ws
 
 
 def distill_forward(logits, teacher_ids, teacher_logits, teacher_lse=None, temperature=1.0, loss=None, stats=None, workspace=None,
                     stream=None):
     """(loss [rows], stats [rows][2]) of fp32 or bf16 rows against the teacher's top logits."""
-    import torch
-    (n, V), dev, f32 = logits.shape, logits.device, torch.float32
-    loss = torch.empty(n, device=dev) if loss is None else loss
-    stats = torch.empty((n, 2), device=dev) if stats is None else stats
-    ws, size = _workspace(workspace, 0 if workspace is not None else lib().ds41_distill_workspace_bytes(n, V), dev)
-    check(lib().ds41_distill_forward(*_teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature),
-                                     _flat(loss, "loss", f32, n), _flat(stats, "stats", f32, 2 * n), ws.data_ptr(), size,
-                                     _stream(stream)), "ds41_distill_forward")
+    args = _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature)
+    loss, stats, loss_p, stats_p, ws = _loss(logits, loss, stats, workspace, stream)
+    check(lib().ds41_distill_forward(*args, loss_p, stats_p, ws[0], ws[1], _stream(stream)), "ds41_distill_forward")
     return loss, stats
 
 
 def _grad(logits, grad):
-    import torch
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad is None else grad
-    if grad.shape != logits.shape:
+    if grad is None:
+        grad = logits.new_empty(logits.shape)
+    elif grad.shape != logits.shape:
         raise ValueError(f"grad has the shape of logits, {tuple(logits.shape)}")
     return grad, _rows(grad, "grad", logits.dtype)
 
 
 def distill_backward(logits, teacher_ids, teacher_logits, stats, grad_loss, teacher_lse=None, temperature=1.0, grad=None, stream=None):
     """The gradient of the logits (grad, which may be logits, or a new tensor)."""
-    import torch
-    n, f32 = logits.shape[0], torch.float32
+    args, f32, n = _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature), _dtypes()[0], logits.shape[0]
     grad, ld_grad = _grad(logits, grad)
-    check(lib().ds41_distill_backward(*_teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature),
-                                      _flat(stats, "stats", f32, 2 * n), _flat(grad_loss, "grad_loss", f32, n), grad.data_ptr(),
+    check(lib().ds41_distill_backward(*args, _flat(stats, "stats", f32, 2 * n), _flat(grad_loss, "grad_loss", f32, n), grad.data_ptr(),
                                       ld_grad, _stream(stream)), "ds41_distill_backward")
     return grad
 
@@ -1303,13 +1331,9 @@ def distill_backward(logits, teacher_ids, teacher_logits, stats, grad_loss, teac
 def distill_step(logits, teacher_ids, teacher_logits, grad_loss, teacher_lse=None, temperature=1.0, loss=None, stats=None, grad=None,
                  workspace=None, stream=None):
     """(loss, stats, grad): distill_forward and distill_backward in one call."""
-    import torch
-    (n, V), dev, f32 = logits.shape, logits.device, torch.float32
-    loss = torch.empty(n, device=dev) if loss is None else loss
-    stats = torch.empty((n, 2), device=dev) if stats is None else stats
+    args = _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature)
     grad, ld_grad = _grad(logits, grad)
-    ws, size = _workspace(workspace, 0 if workspace is not None else lib().ds41_distill_workspace_bytes(n, V), dev)
-    check(lib().ds41_distill_step(*_teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature),
-                                  _flat(grad_loss, "grad_loss", f32, n), _flat(loss, "loss", f32, n), _flat(stats, "stats", f32, 2 * n),
-                                  grad.data_ptr(), ld_grad, ws.data_ptr(), size, _stream(stream)), "ds41_distill_step")
+    loss, stats, loss_p, stats_p, ws = _loss(logits, loss, stats, workspace, stream)
+    check(lib().ds41_distill_step(*args, _flat(grad_loss, "grad_loss", _dtypes()[0], logits.shape[0]), loss_p, stats_p, grad.data_ptr(),
+                                  ld_grad, ws[0], ws[1], _stream(stream)), "ds41_distill_step")
     return loss, stats, grad
