@@ -48,7 +48,7 @@ int ds41_token_counts_commit(uint32_t *counts, uint32_t *seen, int table_rows, i
 /* ---- penalties, biases and grammar masks ---------------------------------------------
  * Logits F32, row s * rows + j of [sequences * rows] for row j of sequence s (a verify step's target rows, or
  * the rows its drafts are drawn from), ld_in apart, to out, ld_out apart. out may be logits (with ld_out ==
- * ld_in; entries that nothing touches are then neither read nor written) and must not overlap it otherwise.
+ * ld_in; entries that nothing touches are then not written) and must not overlap it otherwise.
  * With c the entry's count in the sequence's table row plus its occurrences among the sequence's drafts
  * before row j (drafts int32 [sequences][draft_ld], the first j of them; entries outside the vocabulary are
  * left out), s whether its mark is set or it occurs among those drafts, and penalties[s] = {repetition,
@@ -106,7 +106,7 @@ int ds41_top_logits(const void *logits, int type, size_t ld, int rows, int vocab
  * [rows]; stats F32 [rows][2] = {log sum exp z, log q_r (0 when renormalised)}, which the backward call takes;
  * both 0 for such a row. grad: grad_loss[row] (F32 [rows]) times the derivative, in the logits' type, ld_grad
  * apart; grad may be logits (with ld_grad == ld) and must not overlap it otherwise. k 1 .. 128; temperature
- * > 0. ds41_distill_step is forward and backward in one call, for a grad_loss known beforehand.
+ * 0.01 .. 100. ds41_distill_step is forward and backward in one call, for a grad_loss known beforehand.
  * workspace: ds41_distill_workspace_bytes(rows, vocab) device bytes, 256-byte aligned; calls that share one
  * must be ordered. */
 size_t ds41_distill_workspace_bytes(int rows, int vocab);

@@ -132,7 +132,9 @@ def test_sizes(gpu, V, dtype):
 def test_many_rows_and_strides(gpu, dtype):
     import torch
     dt = getattr(torch, dtype)
-    for n, V, k, T, rest, pad in ((600, 3001, 64, 1.0, True, 0), (300, 33000, 20, 2.0, False, 0), (40, 5000, 16, 1.0, True, 1), (40, 5000, 16, 1.0, False, 8)):
+    for n, V, k, T, rest, pad in ((600, 3001, 64, 1.0, True, 0), (300, 33000, 20, 2.0, False, 0), (40, 5000, 16, 1.0, True, 1), (40, 5000, 16, 1.0, False, 8),
+                                  (3500, 3001, 10, 1.0, True, 1), (800, 16384, 100, 1.0, True, 0), (700, 16385, 5, 1.5, False, 3), (450, 30001, 33, 1.0, True, 0),
+                                  (110, 100003, 64, 1.0, True, 1), (90, 129281, 128, 2.0, False, 0)):
         x, ids, tl, tlse, gl = make(gpu, n, n, V, k, dt, T, rest, pad=pad)
         check(x, ids, tl, tlse, gl, T)
         check(x, ids, tl, tlse, gl, T, in_place=True)
@@ -205,6 +207,35 @@ def test_gradient_against_differences(gpu, rest):
         up, down = (G.distill_forward(x + s * h * v, ids, tl, teacher_lse=tlse)[0].double() for s in (1, -1))
         off = (up - down) / (2 * h) - (grad.double() * v.double()).sum(1)
         assert float(off.abs().max()) <= h * h / 3 + 4 * S(V) / h + 1e-4, float(off.abs().max())
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_rows_held_whole_hold_what_chunks_give(gpu, rest):
+    """Enough bytes that a step keeps its rows in registers: padding, repeated ids, masked, NaN and infinite entries as in
+    few rows, which go in chunks."""
+    import torch
+    import ds41_gfx950 as G
+    for dt, n, V in ((torch.bfloat16, 1200, 9000), (torch.float32, 600, 9001)):
+        x, ids, tl, tlse, gl = make(gpu, 9, n, V, 20, dt, 1.0, rest)
+        keep = torch.zeros_like(x, dtype=torch.bool).scatter_(1, ids.long(), True)
+        keep[:, ::5] = True
+        x[::3] = torch.where(keep[::3], x[::3], torch.finfo(torch.float32).min if dt == torch.float32 else -float("inf"))
+        ids[1, 3:] = -1
+        tl[2, 4:] = -float("inf")
+        ids[4, 6], ids[7], x[10, 77], x[11, int(ids[11, 0])] = ids[4, 0], -1, float("nan"), float("nan")
+        x[12, 5], x[13, int(ids[13, 3])], x[14] = float("inf"), -float("inf"), torch.finfo(torch.float32).min
+        x[15] = -float("inf")
+        x[16, int(ids[16, 1])] = 90.0  # far above what lies outside the set
+        whole = G.distill_step(x, ids, tl, gl, teacher_lse=tlse)
+        for a in range(0, 40, 8):
+            b = a + 8
+            few = G.distill_step(x[a:b], ids[a:b], tl[a:b], gl[a:b], teacher_lse=None if tlse is None else tlse[a:b])
+            for u, v, tol in zip(whole, few, (4 * S(V), 4 * S(V), 2.0 ** -7 if dt == torch.bfloat16 else 1e-4)):
+                u, v = u[a:b].double(), v.double()
+                assert bool((torch.isnan(u) == torch.isnan(v)).all()) and bool((torch.isinf(u) == torch.isinf(v)).all())
+                fin = torch.isfinite(v)
+                # both within the bound of the formula, so within twice that of each other; gradients by their half step
+                assert bool(((u - v).abs()[fin] <= 2 * tol * (1 + v.abs()[fin])).all()), float(((u - v).abs()[fin] / (1 + v.abs()[fin])).max())
 
 
 def test_teacher_is_student(gpu):

@@ -119,6 +119,20 @@ def test_bad_rows_and_strides(gpu):
             check(gpu, y, 10)
 
 
+def test_small_temperature(gpu):
+    """At a temperature of 1e-5 and less one token holds all the mass: lse is max / T, rounded, and its log-probability 0
+    to the sum's bound; 1e-37 overflows max * log2(e) / T."""
+    import torch
+    import ds41_gfx950 as G
+    x = torch.randn(4, 5000, device=gpu) * 3
+    best = x.max(1)
+    for T in (1e-5, 1e-20, 1e-37):
+        ids, values, lse, lp = G.top_logits(x, 3, temperature=T, chosen=best.indices.int())
+        assert torch.equal(ids[:, 0], best.indices.int()) and torch.equal(values[:, 0], best.values)
+        want = best.values.double() / T
+        assert bool(((lse.double() - want).abs() <= 2.0 ** -22 * want.abs()).all()) and float(lp.abs().max()) <= lse_bound(5000, 0)
+
+
 def test_longest_vocabulary(gpu):
     import torch
     V = 1 << 20

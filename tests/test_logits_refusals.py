@@ -99,7 +99,7 @@ STEP = dict(TEACHER, grad_loss=P, loss=P, stats=P, grad=P + (1 << 16), ld_grad=1
 @pytest.mark.parametrize("change", [
     dict(logits=None), dict(type=2), dict(type=-1), dict(ld=999), dict(rows=0), dict(rows=65536), dict(vocab=0), dict(ids=None),
     dict(tlogits=None), dict(k=0), dict(k=129), dict(temperature=0.0), dict(temperature=float("inf")), dict(temperature=float("nan")),
-    dict(stats=None),
+    dict(temperature=0.001), dict(temperature=1000.0), dict(temperature=-1.0), dict(stats=None),
 ])
 def test_distill_refusals(change):
     for name, args in (("distill_forward", FORWARD), ("distill_backward", BACKWARD), ("distill_step", STEP)):
