@@ -83,7 +83,8 @@ int ds41_logits_control(const float *logits, size_t ld_in, float *out, size_t ld
  * lse F32 [rows] = log sum exp(x / temperature); logprob F32 [rows] = x[chosen] / temperature - lse for
  * chosen int32 [rows], NaN where that is outside the vocabulary. ids and values may both be NULL, so may lse,
  * and chosen with logprob. -infinity is an ordinary smallest value; a row with NaN or +infinity gives ids -1
- * and NaN. k 1 .. 128 and at most vocab; temperature > 0.
+ * and NaN. k 1 .. 128 and at most vocab; temperature from
+ * FLT_MIN to 1e38.
  * workspace: ds41_top_logits_workspace_bytes(rows, vocab, k) device bytes, 256-byte aligned; calls that
  * share one must be ordered. */
 size_t ds41_top_logits_workspace_bytes(int rows, int vocab, int k);

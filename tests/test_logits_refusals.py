@@ -138,3 +138,9 @@ def test_binding_refuses_wrong_tensors():
         G.top_logits(z, 5, ids=torch.zeros(4, 5), workspace=torch.zeros(1))
     with pytest.raises(ValueError):
         G.token_counts_commit(torch.zeros(1, 9, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32), 9, torch.zeros(9, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("temperature", [1e-38, 1e-45, 2e38, 3.4e38])
+def test_top_refuses_temperatures_whose_scale_is_not_normal(temperature):
+    """log2(e) / T is infinite below FLT_MIN's reach and not a normal number above 1e38."""
+    assert call("top_logits", TOP, temperature=temperature) == INVALID
