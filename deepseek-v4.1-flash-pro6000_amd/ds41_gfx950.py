@@ -476,6 +476,32 @@ def _flat(t, what, dtype, n):
     raise ValueError(f"{what}: {n} contiguous elements of {dtype}, not {tuple(t.shape)} {t.dtype}")
 
 
+def _stream_of(stream, first, *others):
+    """hipStream_t of a torch stream, or of the current one, on the device that every tensor is on."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {t.device} and {first.device}")
+    if dev < 0:
+        raise ValueError(f"tensors on {first.device}")
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    if dev != (_torch._C._cuda_getDevice() if stream is None else stream.device_index):
+        raise ValueError(f"tensors on {first.device}, the stream is on another device")
+    return _torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+
+
+def _new(stream, like, shape, dtype):
+    """A tensor for a call on `stream`: of that stream's memory, which no earlier work of another stream still uses."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    import torch
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
 def dense_bf16_workspace_bytes(M, N, K):
     return lib().ds41_dense_bf16_workspace_bytes(M, N, K)
 
@@ -489,7 +515,7 @@ def dense_bf16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=N
     if Kw != K:
         raise ValueError(f"x has {K} columns, w {Kw}")
     if out is None:
-        out = x.new_empty((M, N), dtype=out_dtype or bf16)
+        out = _new(stream, x, (M, N), out_dtype or bf16)
     elif out.shape != (M, N):
         raise ValueError(f"out has shape {(M, N)}, not {tuple(out.shape)}")
     ldr, res = 0, None
@@ -499,7 +525,8 @@ def dense_bf16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=N
         ldr, res = _rows(residual, "residual", out.dtype), residual.data_ptr()
     ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
     check(lib().ds41_dense_bf16(x.data_ptr(), ldx, w.data_ptr(), ldw, _flat(bias, "bias", f32, N), res, ldr, out.data_ptr(),
-                                _rows(out, "out"), _type(out), M, N, K, ACTS[act], ws, size, _stream(stream)), "ds41_dense_bf16")
+                                _rows(out, "out"), _type(out), M, N, K, ACTS[act], ws, size,
+                                _stream_of(stream, x, w, bias, residual, out, workspace)), "ds41_dense_bf16")
     return out
 
 
@@ -1200,8 +1227,8 @@ def token_counts_clear(counts, seen, vocab, table_index=None, stream=None):
     """Empties every table row, or the ones in table_index."""
     c, s, rows = _table(counts, seen, vocab)
     n = rows if table_index is None else table_index.numel()
-    check(lib().ds41_token_counts_clear(c, s, rows, vocab, _flat(table_index, "table_index", _dtypes()[2], n), n, _stream(stream)),
-          "ds41_token_counts_clear")
+    check(lib().ds41_token_counts_clear(c, s, rows, vocab, _flat(table_index, "table_index", _dtypes()[2], n), n,
+                                        _stream_of(stream, counts, seen, table_index)), "ds41_token_counts_clear")
 
 
 def token_counts_add(counts, seen, vocab, tokens, offsets, table_index=None, generated=True, stream=None):
@@ -1211,7 +1238,8 @@ def token_counts_add(counts, seen, vocab, tokens, offsets, table_index=None, gen
     n = offsets.numel() - 1
     check(lib().ds41_token_counts_add(c, s, rows, vocab, _flat(table_index, "table_index", _dtypes()[2], n),
                                       _flat(tokens, "tokens", _dtypes()[2], 0), _flat(offsets, "offsets", _dtypes()[2], 2), n,
-                                      tokens.numel(), int(generated), _stream(stream)), "ds41_token_counts_add")
+                                      tokens.numel(), int(generated), _stream_of(stream, counts, seen, tokens, offsets, table_index)),
+          "ds41_token_counts_add")
 
 
 def token_counts_commit(counts, seen, vocab, results, n=1, table_index=None, stream=None):
@@ -1220,7 +1248,7 @@ def token_counts_commit(counts, seen, vocab, results, n=1, table_index=None, str
     if results.nbytes < n * ctypes.sizeof(SparkResult) or not results.is_contiguous():
         raise ValueError(f"results: {n} contiguous ds41_spark_result")
     check(lib().ds41_token_counts_commit(c, s, rows, vocab, _flat(table_index, "table_index", _dtypes()[2], n), results.data_ptr(), n,
-                                         _stream(stream)), "ds41_token_counts_commit")
+                                         _stream_of(stream, counts, seen, results, table_index)), "ds41_token_counts_commit")
 
 
 LOWEST = -3.4028234663852886e38  # a masked value that the samplers take (they reject rows with infinities)
@@ -1252,36 +1280,36 @@ def logits_control(logits, rows=1, counts=None, seen=None, table_index=None, dra
         logits.data_ptr(), ld_in, out.data_ptr(), ld_out, S, rows, V, c, s, table_rows, _flat(table_index, "table_index", i32, S), d, draft_ld,
         _flat(penalties, "penalties", f32, 3 * S), _flat(bias_ids, "bias_ids", i32, 0), _flat(bias_values, "bias_values", f32, total),
         _flat(bias_offsets, "bias_offsets", i32, S + 1), total, mask_p, mask_ld, mask_rows, _flat(mask_index, "mask_index", i32, n),
-        masked_value, _stream(stream)), "ds41_logits_control")
+        masked_value, _stream_of(stream, logits, out, counts, seen, table_index, drafts, penalties, bias_ids, bias_values, bias_offsets, mask,
+                                 mask_index)), "ds41_logits_control")
     return out
 
 
 def _workspace(t, need, like, stream):
-    """(address, bytes, tensor) of a workspace, of a new one of need() bytes where none is given, whose memory torch's
-    allocator keeps for the stream that the call uses."""
+    """A workspace, or a new one of need() bytes where none is given."""
     if t is None:
         import torch
-        t = torch.empty(max(need(), 1), dtype=torch.uint8, device=like.device)
-        if stream is not None:
-            t.record_stream(stream)
-    return t.data_ptr(), t.nbytes, t
+        t = _new(stream, like, (max(need(), 1),), torch.uint8)
+    return t
 
 
 def top_logits(logits, k, temperature=1.0, chosen=None, ids=None, values=None, lse=None, logprob=None, workspace=None, stream=None):
     """(ids [rows][k], values [rows][k], lse [rows], logprob [rows] or None without chosen) of fp32 or bf16 rows."""
     f32, _, i32 = _dtypes()
     ld, (n, V) = _rows(logits, "logits"), logits.shape
-    ids = logits.new_empty((n, k), dtype=i32) if ids is None else ids
-    values = logits.new_empty((n, k), dtype=f32) if values is None else values
-    lse = logits.new_empty(n, dtype=f32) if lse is None else lse
+    ids = _new(stream, logits, (n, k), i32) if ids is None else ids
+    values = _new(stream, logits, (n, k), f32) if values is None else values
+    lse = _new(stream, logits, (n,), f32) if lse is None else lse
     lp = None
     if chosen is not None:
-        logprob = logits.new_empty(n, dtype=f32) if logprob is None else logprob
+        logprob = _new(stream, logits, (n,), f32) if logprob is None else logprob
         lp = _flat(logprob, "logprob", f32, n)
-    ws, size, keep = _workspace(workspace, lambda: lib().ds41_top_logits_workspace_bytes(n, V, k), logits, stream)
+    ws = _workspace(workspace, lambda: lib().ds41_top_logits_workspace_bytes(n, V, k), logits, stream)
     check(lib().ds41_top_logits(logits.data_ptr(), _type(logits), ld, n, V, k, temperature, _flat(ids, "ids", i32, n * k),
                                 _flat(values, "values", f32, n * k), _flat(lse, "lse", f32, n), _flat(chosen, "chosen", i32, n), lp,
-                                ws, size, _stream(stream)), "ds41_top_logits")
+                                ws.data_ptr(), ws.nbytes,
+                                _stream_of(stream, logits, ids, values, lse, chosen, logprob if chosen is not None else None, ws)),
+          "ds41_top_logits")
     return ids, values, lse, logprob if chosen is not None else None
 
 
@@ -1294,10 +1322,10 @@ def _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature):
 
 
 def _loss(logits, loss, stats, workspace, stream):
-    """loss, stats and workspace of a forward call, with their addresses."""
+    """loss, stats, their addresses, and the workspace of a forward call."""
     f32, (n, V) = _dtypes()[0], logits.shape
-    loss = logits.new_empty(n, dtype=f32) if loss is None else loss
-    stats = logits.new_empty((n, 2), dtype=f32) if stats is None else stats
+    loss = _new(stream, logits, (n,), f32) if loss is None else loss
+    stats = _new(stream, logits, (n, 2), f32) if stats is None else stats
     ws = _workspace(workspace, lambda: lib().ds41_distill_workspace_bytes(n, V), logits, stream)
     return loss, stats, _flat(loss, "loss", f32, n), _flat(stats, "stats", f32, 2 * n), ws
 
@@ -1307,13 +1335,15 @@ def distill_forward(logits, teacher_ids, teacher_logits, teacher_lse=None, tempe
     """(loss [rows], stats [rows][2]) of fp32 or bf16 rows against the teacher's top logits."""
     args = _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature)
     loss, stats, loss_p, stats_p, ws = _loss(logits, loss, stats, workspace, stream)
-    check(lib().ds41_distill_forward(*args, loss_p, stats_p, ws[0], ws[1], _stream(stream)), "ds41_distill_forward")
+    check(lib().ds41_distill_forward(*args, loss_p, stats_p, ws.data_ptr(), ws.nbytes,
+                                     _stream_of(stream, logits, teacher_ids, teacher_logits, teacher_lse, loss, stats, ws)),
+          "ds41_distill_forward")
     return loss, stats
 
 
-def _grad(logits, grad):
+def _grad(logits, grad, stream):
     if grad is None:
-        grad = logits.new_empty(logits.shape)
+        grad = _new(stream, logits, logits.shape, logits.dtype)
     elif grad.shape != logits.shape:
         raise ValueError(f"grad has the shape of logits, {tuple(logits.shape)}")
     return grad, _rows(grad, "grad", logits.dtype)
@@ -1322,9 +1352,10 @@ def _grad(logits, grad):
 def distill_backward(logits, teacher_ids, teacher_logits, stats, grad_loss, teacher_lse=None, temperature=1.0, grad=None, stream=None):
     """The gradient of the logits (grad, which may be logits, or a new tensor)."""
     args, f32, n = _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature), _dtypes()[0], logits.shape[0]
-    grad, ld_grad = _grad(logits, grad)
+    grad, ld_grad = _grad(logits, grad, stream)
     check(lib().ds41_distill_backward(*args, _flat(stats, "stats", f32, 2 * n), _flat(grad_loss, "grad_loss", f32, n), grad.data_ptr(),
-                                      ld_grad, _stream(stream)), "ds41_distill_backward")
+                                      ld_grad, _stream_of(stream, logits, teacher_ids, teacher_logits, teacher_lse, stats, grad_loss, grad)),
+          "ds41_distill_backward")
     return grad
 
 
@@ -1332,8 +1363,10 @@ def distill_step(logits, teacher_ids, teacher_logits, grad_loss, teacher_lse=Non
                  workspace=None, stream=None):
     """(loss, stats, grad): distill_forward and distill_backward in one call."""
     args = _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature)
-    grad, ld_grad = _grad(logits, grad)
+    grad, ld_grad = _grad(logits, grad, stream)
     loss, stats, loss_p, stats_p, ws = _loss(logits, loss, stats, workspace, stream)
     check(lib().ds41_distill_step(*args, _flat(grad_loss, "grad_loss", _dtypes()[0], logits.shape[0]), loss_p, stats_p, grad.data_ptr(),
-                                  ld_grad, ws[0], ws[1], _stream(stream)), "ds41_distill_step")
+                                  ld_grad, ws.data_ptr(), ws.nbytes,
+                                  _stream_of(stream, logits, teacher_ids, teacher_logits, teacher_lse, grad_loss, loss, stats, grad, ws)),
+          "ds41_distill_step")
     return loss, stats, grad

@@ -76,3 +76,42 @@ def test_answer_path(gpu):
     assert np.array_equal(counts[0].cpu().numpy(), want) and G.take_status() == 0
     marks = np.unpackbits(seen.cpu().numpy().view(np.uint8), bitorder="little")[:V].astype(bool)
     assert np.array_equal(marks, (want > 0) | np.isin(np.arange(V), prompt.cpu().numpy()))
+
+
+def test_host_tensors_among_device_tensors_are_refused(gpu):
+    import torch
+    import ds41_gfx950 as G
+    x, w = torch.zeros(4, 64, device=gpu).bfloat16(), torch.zeros(32, 64, device=gpu).bfloat16()
+    z, pen = torch.zeros(4, 96, device=gpu), torch.ones(12)
+    ids, t = torch.zeros(4, 5, dtype=torch.int32, device=gpu), torch.zeros(4, 5, device=gpu)
+    for f in (lambda: G.dense_bf16(x, w.cpu()), lambda: G.dense_bf16(x, w, bias=torch.zeros(32)), lambda: G.logits_control(z, penalties=pen),
+              lambda: G.top_logits(z, 5, chosen=torch.zeros(4, dtype=torch.int32)), lambda: G.distill_forward(z, ids.cpu(), t),
+              lambda: G.distill_step(z, ids, t, torch.zeros(4))):
+        with pytest.raises(ValueError, match="tensors on"):
+            f()
+
+
+def test_tensors_made_for_another_stream_are_of_its_memory(gpu):
+    """A call on a stream of its own, right after tensors of the sizes it makes were freed with work of the current
+    stream still to come on them: its results are not written over, and equal the current stream's."""
+    import torch
+    import ds41_gfx950 as G
+    rng = torch.Generator(device="cpu").manual_seed(5)
+    x, w = torch.randn(64, 512, generator=rng).to(gpu).bfloat16(), torch.randn(4096, 512, generator=rng).to(gpu).bfloat16()
+    z = torch.randn(64, 4096, generator=rng).to(gpu)
+    t, ids = torch.topk(z, 20)
+    ids, gl = ids.int(), torch.ones(64, device=gpu)
+    want = [G.dense_bf16(x, w), *G.top_logits(z, 20)[:3], *G.distill_step(z, ids, t, gl)]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for o in want:  # written late by the current stream, and free at once
+            held = [torch.empty_like(o) for _ in range(4)]
+            for h in held:
+                for _ in range(20):
+                    h.fill_(3)
+            del held, h
+        got = [G.dense_bf16(x, w, stream=s), *G.top_logits(z, 20, stream=s)[:3], *G.distill_step(z, ids, t, gl, stream=s)]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)

@@ -144,3 +144,19 @@ def test_binding_refuses_wrong_tensors():
 def test_top_refuses_temperatures_whose_scale_is_not_normal(temperature):
     """log2(e) / T is infinite below FLT_MIN's reach and not a normal number above 1e38."""
     assert call("top_logits", TOP, temperature=temperature) == INVALID
+
+
+def test_binding_refuses_host_tensors():
+    """A host address in a kernel's arguments would fault: well-formed calls on host tensors raise before the entry."""
+    import torch
+    bf16, i32 = torch.bfloat16, torch.int32
+    z, counts, seen = torch.zeros(4, 96), torch.zeros(4, 96, dtype=i32), torch.zeros(4, 3, dtype=i32)
+    ids, t, one = torch.zeros(4, 5, dtype=i32), torch.zeros(4, 5), torch.zeros(4)
+    for f in (lambda: G.dense_bf16(torch.zeros(4, 64, dtype=bf16), torch.zeros(32, 64, dtype=bf16)),
+              lambda: G.logits_control(z, counts=counts, seen=seen), lambda: G.token_counts_clear(counts, seen, 96),
+              lambda: G.token_counts_add(counts, seen, 96, ids.flatten(), torch.zeros(5, dtype=i32)),
+              lambda: G.token_counts_commit(counts, seen, 96, torch.zeros(40, dtype=torch.uint8)), lambda: G.top_logits(z, 5),
+              lambda: G.distill_forward(z, ids, t), lambda: G.distill_backward(z, ids, t, torch.zeros(4, 2), one),
+              lambda: G.distill_step(z, ids, t, one)):
+        with pytest.raises(ValueError, match="tensors on cpu"):
+            f()
