@@ -102,7 +102,9 @@ int ds41_top_logits(const void *logits, int type, size_t ld, int rows, int vocab
  *         matched with q_r, the student's mass outside the set (0 where the set is the whole vocabulary)
  *   loss = sum p_i (log p_i - log q_i) [+ p_r (log p_r - log q_r)]
  *   d loss / d logit_j = (q_j - p_j) / temperature in the set, and outside it q_j / temperature
- *         [times 1 - p_r / q_r]
+ *         [times 1 - p_r / q_r, whose p_r q_j / q_r stays of p_r's size where the set holds nearly all of q]
+ * Where every logit outside the set is -infinity, log q_r is -infinity, the loss +infinity if p_r > 0, and the gradient
+ * outside 0. What a grammar masks of the student belongs in the renormalised form, or the teacher's rest pulls on it.
  * A row with nothing in its set has loss 0 and gradient 0 whatever its logits hold (padding). loss F32
  * [rows]; stats F32 [rows][2] = {log sum exp z, log q_r (0 when renormalised)}, which the backward call takes;
  * both 0 for such a row. grad: grad_loss[row] (F32 [rows]) times the derivative, in the logits' type, ld_grad
