@@ -138,7 +138,7 @@ def check(x, ids, tl, tlse, gl, T, dtype):
             near(g, grad, tol, what + " gradient")
 
 
-@pytest.mark.parametrize("rest", [True])
+@pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("path", list(ROWS))
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("T", [0.01, 0.1, 1.0, 100.0])
@@ -147,7 +147,7 @@ def test_sets_far_from_the_rest(gpu, T, dtype, path, rest):
     check(*make(gpu, int(T * 100) + n, n, V, k, dtype, T, rest), T, dtype)
 
 
-@pytest.mark.parametrize("rest", [True])
+@pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("path", list(ROWS))
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_left_out_and_repeated_entries_of_such_rows(gpu, dtype, path, rest):
