@@ -85,8 +85,8 @@ int ds41_logits_control(const float *logits, size_t ld_in, float *out, size_t ld
  * and chosen with logprob. -infinity is an ordinary smallest value; a row with NaN or +infinity gives ids -1
  * and NaN. k 1 .. 128 and at most vocab; temperature from
  * FLT_MIN to 1e38.
- * workspace: ds41_top_logits_workspace_bytes(rows, vocab, k) device bytes, 256-byte aligned; calls that
- * share one must be ordered. */
+ * workspace: ds41_top_logits_workspace_bytes(rows, vocab, k) device bytes, 256-byte aligned, which cover every call of
+ * no more rows, entries and k; calls that share one must be ordered. */
 size_t ds41_top_logits_workspace_bytes(int rows, int vocab, int k);
 int ds41_top_logits(const void *logits, int type, size_t ld, int rows, int vocab, int k, float temperature,
                     int32_t *ids, float *values, float *lse, const int32_t *chosen, float *logprob,
@@ -112,8 +112,8 @@ int ds41_top_logits(const void *logits, int type, size_t ld, int rows, int vocab
  * where that sum is above 8,192. grad: grad_loss[row] (F32 [rows]) times the derivative, in the logits' type, ld_grad
  * apart; grad may be logits (with ld_grad == ld) and must not overlap it otherwise. k 1 .. 128; temperature
  * 0.01 .. 100. ds41_distill_step is forward and backward in one call, for a grad_loss known beforehand.
- * workspace: ds41_distill_workspace_bytes(rows, vocab) device bytes, 256-byte aligned; calls that share one
- * must be ordered. */
+ * workspace: ds41_distill_workspace_bytes(rows, vocab) device bytes, 256-byte aligned, which cover every call of no
+ * more rows and entries; calls that share one must be ordered. */
 size_t ds41_distill_workspace_bytes(int rows, int vocab);
 int ds41_distill_forward(const void *logits, int type, size_t ld, int rows, int vocab,
                          const int32_t *teacher_ids, const float *teacher_logits, int k,

@@ -382,8 +382,9 @@ int ds41_dense_shared_act(const void *gate_bf16, const void *up_bf16, void *z_bf
  * in the reference's own kernels (its bf16 head and projections are library and generated code,
  * components/fuse-head, components/dense/include/ds41/dense.h:28).
  * workspace (nullable): ds41_dense_bf16_workspace_bytes(M, N, K) device bytes, 256-byte aligned, let a product
- * of few output tiles be split over K (partial sums in a fixed order: the same bits every call). Without it,
- * or with less, the product is not split; calls that share one must be ordered. */
+ * of few output tiles be split over K (partial sums in a fixed order: the same bits every call). The size covers
+ * every product of no more rows with the same N and K. Without it, or with less than a product's parts need, the
+ * product is not split; calls that share one must be ordered. */
 enum { DS41_ACT_NONE = 0, DS41_ACT_RELU = 1, DS41_ACT_SILU = 2, DS41_ACT_GELU = 3 /* exact, with erf */ };
 size_t ds41_dense_bf16_workspace_bytes(int M, int N, int K);
 int ds41_dense_bf16(const void *x_bf16, size_t ldx, const void *w_bf16, size_t ldw, const float *bias,
