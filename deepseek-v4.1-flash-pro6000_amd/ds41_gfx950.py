@@ -476,6 +476,17 @@ def _flat(t, what, dtype, n):
     raise ValueError(f"{what}: {n} contiguous elements of {dtype}, not {tuple(t.shape)} {t.dtype}")
 
 
+def _wide(t, what, dtype, n, width):
+    """Address of n contiguous rows of width elements (at least n; all in one dimension, exactly), or null."""
+    if t is None:
+        return None
+    if t.dtype is dtype and t.is_contiguous():
+        shape = t.shape
+        if shape[-1] == width and t.numel() >= n * width if len(shape) > 1 else t.numel() == n * width:
+            return t.data_ptr()
+    raise ValueError(f"{what}: {n} contiguous rows of {width} {dtype}, not {tuple(t.shape)} {t.dtype}")
+
+
 def _stream_of(stream, first, *others):
     """hipStream_t of a torch stream, or of the current one, on the device that every tensor is on."""
     dev = first.get_device()
@@ -1220,7 +1231,10 @@ def token_counts(table_rows, vocab, device="cuda"):
 
 def _table(counts, seen, vocab):
     rows, i32 = (counts if counts is not None else seen).shape[0], _dtypes()[2]
-    return _flat(counts, "counts", i32, rows * vocab), _flat(seen, "seen", i32, rows * ((vocab + 31) // 32)), rows
+    for t in (counts, seen):
+        if t is not None and len(t.shape) != 2:
+            raise ValueError(f"a token table is two matrices, not {tuple(t.shape)}")
+    return _wide(counts, "counts", i32, rows, vocab), _wide(seen, "seen", i32, rows, (vocab + 31) // 32), rows
 
 
 def token_counts_clear(counts, seen, vocab, table_index=None, stream=None):
@@ -1276,9 +1290,11 @@ def logits_control(logits, rows=1, counts=None, seen=None, table_index=None, dra
         total = bias_ids.numel()
     if mask is not None:
         mask_p, mask_ld, mask_rows = mask.data_ptr(), _rows(mask, "mask", i32), mask.shape[0]
+        if mask.shape[1] < (V + 31) // 32:
+            raise ValueError(f"mask: rows of {(V + 31) // 32} words, not {tuple(mask.shape)}")
     check(lib().ds41_logits_control(
         logits.data_ptr(), ld_in, out.data_ptr(), ld_out, S, rows, V, c, s, table_rows, _flat(table_index, "table_index", i32, S), d, draft_ld,
-        _flat(penalties, "penalties", f32, 3 * S), _flat(bias_ids, "bias_ids", i32, 0), _flat(bias_values, "bias_values", f32, total),
+        _wide(penalties, "penalties", f32, S, 3), _flat(bias_ids, "bias_ids", i32, 0), _flat(bias_values, "bias_values", f32, total),
         _flat(bias_offsets, "bias_offsets", i32, S + 1), total, mask_p, mask_ld, mask_rows, _flat(mask_index, "mask_index", i32, n),
         masked_value, _stream_of(stream, logits, out, counts, seen, table_index, drafts, penalties, bias_ids, bias_values, bias_offsets, mask,
                                  mask_index)), "ds41_logits_control")
@@ -1305,8 +1321,8 @@ def top_logits(logits, k, temperature=1.0, chosen=None, ids=None, values=None, l
         logprob = _new(stream, logits, (n,), f32) if logprob is None else logprob
         lp = _flat(logprob, "logprob", f32, n)
     ws = _workspace(workspace, lambda: lib().ds41_top_logits_workspace_bytes(n, V, k), logits, stream)
-    check(lib().ds41_top_logits(logits.data_ptr(), _type(logits), ld, n, V, k, temperature, _flat(ids, "ids", i32, n * k),
-                                _flat(values, "values", f32, n * k), _flat(lse, "lse", f32, n), _flat(chosen, "chosen", i32, n), lp,
+    check(lib().ds41_top_logits(logits.data_ptr(), _type(logits), ld, n, V, k, temperature, _wide(ids, "ids", i32, n, k),
+                                _wide(values, "values", f32, n, k), _flat(lse, "lse", f32, n), _flat(chosen, "chosen", i32, n), lp,
                                 ws.data_ptr(), ws.nbytes,
                                 _stream_of(stream, logits, ids, values, lse, chosen, logprob if chosen is not None else None, ws)),
           "ds41_top_logits")
@@ -1317,8 +1333,8 @@ def _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature):
     """The arguments that the distillation calls share."""
     f32, _, i32 = _dtypes()
     (n, V), k = logits.shape, teacher_ids.shape[-1]
-    return (logits.data_ptr(), _type(logits), _rows(logits, "logits"), n, V, _flat(teacher_ids, "teacher_ids", i32, n * k),
-            _flat(teacher_logits, "teacher_logits", f32, n * k), k, _flat(teacher_lse, "teacher_lse", f32, n), temperature)
+    return (logits.data_ptr(), _type(logits), _rows(logits, "logits"), n, V, _wide(teacher_ids, "teacher_ids", i32, n, k),
+            _wide(teacher_logits, "teacher_logits", f32, n, k), k, _flat(teacher_lse, "teacher_lse", f32, n), temperature)
 
 
 def _loss(logits, loss, stats, workspace, stream):
@@ -1327,7 +1343,7 @@ def _loss(logits, loss, stats, workspace, stream):
     loss = _new(stream, logits, (n,), f32) if loss is None else loss
     stats = _new(stream, logits, (n, 2), f32) if stats is None else stats
     ws = _workspace(workspace, lambda: lib().ds41_distill_workspace_bytes(n, V), logits, stream)
-    return loss, stats, _flat(loss, "loss", f32, n), _flat(stats, "stats", f32, 2 * n), ws
+    return loss, stats, _flat(loss, "loss", f32, n), _wide(stats, "stats", f32, n, 2), ws
 
 
 def distill_forward(logits, teacher_ids, teacher_logits, teacher_lse=None, temperature=1.0, loss=None, stats=None, workspace=None,
@@ -1353,7 +1369,7 @@ def distill_backward(logits, teacher_ids, teacher_logits, stats, grad_loss, teac
     """The gradient of the logits (grad, which may be logits, or a new tensor)."""
     args, f32, n = _teacher(logits, teacher_ids, teacher_logits, teacher_lse, temperature), _dtypes()[0], logits.shape[0]
     grad, ld_grad = _grad(logits, grad, stream)
-    check(lib().ds41_distill_backward(*args, _flat(stats, "stats", f32, 2 * n), _flat(grad_loss, "grad_loss", f32, n), grad.data_ptr(),
+    check(lib().ds41_distill_backward(*args, _wide(stats, "stats", f32, n, 2), _flat(grad_loss, "grad_loss", f32, n), grad.data_ptr(),
                                       ld_grad, _stream_of(stream, logits, teacher_ids, teacher_logits, teacher_lse, stats, grad_loss, grad)),
           "ds41_distill_backward")
     return grad

@@ -160,3 +160,35 @@ def test_binding_refuses_host_tensors():
               lambda: G.distill_step(z, ids, t, one)):
         with pytest.raises(ValueError, match="tensors on cpu"):
             f()
+
+
+def test_binding_refuses_rows_of_another_width():
+    """Enough elements, but in rows of another width, which would be read as other rows' elements. The calls are refused by
+    shape, before the tensors' device is looked at."""
+    import torch
+    i32 = torch.int32
+    z, ids, t, one = torch.zeros(4, 96), torch.zeros(4, 5, dtype=i32), torch.zeros(4, 5), torch.zeros(4)
+    counts, seen, bits = torch.zeros(4, 96, dtype=i32), torch.zeros(4, 3, dtype=i32), torch.zeros(4, 6, dtype=i32)
+    padded, padded_seen = torch.zeros(4, 101, dtype=i32), torch.zeros(4, 4, dtype=i32)  # of a padded vocabulary
+    tokens, offsets, results = torch.zeros(5, dtype=i32), torch.zeros(5, dtype=i32), torch.zeros(160, dtype=torch.uint8)
+    wrong = [lambda: G.logits_control(z, counts=padded, seen=seen), lambda: G.logits_control(z, counts=counts, seen=padded_seen),
+             lambda: G.logits_control(z, counts=padded), lambda: G.logits_control(z, seen=padded_seen),
+             lambda: G.logits_control(z, counts=counts.flatten()), lambda: G.logits_control(z, penalties=torch.zeros(4, 4)),
+             lambda: G.logits_control(z, penalties=torch.zeros(13)), lambda: G.logits_control(z, mask=bits[:, :2]),
+             lambda: G.top_logits(z, 5, ids=torch.zeros(4, 8, dtype=i32)), lambda: G.top_logits(z, 5, values=torch.zeros(5, 6)),
+             lambda: G.distill_forward(z, ids, torch.zeros(4, 8)), lambda: G.distill_forward(z, torch.zeros(4, 8, dtype=i32), t),
+             lambda: G.distill_forward(z, ids, t, stats=torch.zeros(4, 3)), lambda: G.distill_backward(z, ids, t, torch.zeros(4, 3), one),
+             lambda: G.distill_step(z, ids, torch.zeros(4, 8), one), lambda: G.distill_step(z, ids, t, one, stats=torch.zeros(3, 4))]
+    for c, s in ((padded, seen), (counts, padded_seen)):
+        wrong += [lambda c=c, s=s: G.token_counts_clear(c, s, 96), lambda c=c, s=s: G.token_counts_add(c, s, 96, tokens, offsets),
+                  lambda c=c, s=s: G.token_counts_commit(c, s, 96, results, n=4)]
+    for f in wrong:
+        with pytest.raises(ValueError) as e:
+            f()
+        assert "tensors on" not in str(e.value)
+    # more rows than the call has, and rows in one dimension, are what they were; the tensors' device is what is refused then
+    for f in (lambda: G.logits_control(z[:2], counts=counts, seen=seen, penalties=torch.zeros(4, 3)),
+              lambda: G.logits_control(z, penalties=torch.zeros(12), mask=bits), lambda: G.distill_step(z[:1], ids[0], t[0], one),
+              lambda: G.distill_step(z[:3], ids, t, one), lambda: G.top_logits(z[:3], 5, ids=ids, values=t)):
+        with pytest.raises(ValueError, match="tensors on cpu"):
+            f()
