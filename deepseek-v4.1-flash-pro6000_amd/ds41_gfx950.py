@@ -7,6 +7,7 @@ Every call raises if the library is missing or returns a HIP error: there is
 no CPU fallback.
 """
 import ctypes
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -513,13 +514,14 @@ def _new(stream, like, shape, dtype):
         return like.new_empty(shape, dtype=dtype)
 
 
+@functools.lru_cache(4096)  # 6 us for 4,096 rows
 def dense_bf16_workspace_bytes(M, N, K):
     return lib().ds41_dense_bf16_workspace_bytes(M, N, K)
 
 
 def dense_bf16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=None, workspace=None, stream=None):
     """act(x w^T + bias) + residual, x bf16 [M][K], w bf16 [N][K], into out (or a new tensor of out_dtype,
-    bfloat16 by default)."""
+    bfloat16 by default). Without a workspace a product that is split over K gets one of its own."""
     f32, bf16, _ = _dtypes()
     ldx, ldw = _rows(x, "x", bf16), _rows(w, "w", bf16)
     (M, K), (N, Kw) = x.shape, w.shape
@@ -534,6 +536,10 @@ def dense_bf16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=N
         if residual.shape != (M, N):
             raise ValueError(f"residual has shape {(M, N)}, not {tuple(residual.shape)}")
         ldr, res = _rows(residual, "residual", out.dtype), residual.data_ptr()
+    if workspace is None:
+        need = dense_bf16_workspace_bytes(M, N, K)
+        if need:
+            workspace = _workspace(None, lambda: need, x, stream)
     ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
     check(lib().ds41_dense_bf16(x.data_ptr(), ldx, w.data_ptr(), ldw, _flat(bias, "bias", f32, N), res, ldr, out.data_ptr(),
                                 _rows(out, "out"), _type(out), M, N, K, ACTS[act], ws, size,

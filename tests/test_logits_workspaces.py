@@ -67,3 +67,29 @@ def test_smaller_calls_in_the_largest_ones_workspace(gpu):
     for m in (1, 33, 64, 65, 100, 128, 129, 190, 256, 300, 511, 600):
         # with room for whatever parts it takes: the same parts, so the same bits
         assert torch.equal(G.dense_bf16(h[:m], w, workspace=ws), G.dense_bf16(h[:m], w, workspace=big)), m
+
+
+@pytest.mark.gpu
+def test_a_product_without_a_workspace_makes_its_own(gpu):
+    """The same parts, so the same bits, as with a workspace, on the current stream, on another and in a graph."""
+    import torch
+    K = 4096
+    s = torch.cuda.Stream()
+    for M, N in ((1, 4096), (33, 4096), (64, 4096), (100, 2881), (128, 5120), (200, 640), (512, 4096)):
+        x, w = torch.randn(M, K, device=gpu).bfloat16(), torch.randn(N, K, device=gpu).bfloat16() * 0.02
+        ws = torch.empty(max(1, G.dense_bf16_workspace_bytes(M, N, K)), dtype=torch.uint8, device=gpu)
+        want = G.dense_bf16(x, w, out_dtype=torch.float32, workspace=ws)
+        assert torch.equal(G.dense_bf16(x, w, out_dtype=torch.float32), want)
+        torch.cuda.synchronize()
+        got = G.dense_bf16(x, w, out_dtype=torch.float32, stream=s)
+        s.synchronize()
+        assert torch.equal(got, want)
+        y, g = torch.empty_like(want), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            G.dense_bf16(x, w, out=y)
+        for i in range(3):
+            x.copy_(torch.randn(M, K, device=gpu))
+            y.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, G.dense_bf16(x, w, out_dtype=torch.float32, workspace=ws))
