@@ -81,7 +81,8 @@ int ds41_logits_control(const float *logits, size_t ld_in, float *out, size_t ld
  * For every row of logits (type DS41_TYPE_*, [rows] of ld): its k largest entries in descending order, equal
  * ones by ascending id (-0 equals +0, and is given as +0), as ids int32 [rows][k] and values F32 [rows][k];
  * lse F32 [rows] = log sum exp(x / temperature); logprob F32 [rows] = x[chosen] / temperature - lse for
- * chosen int32 [rows], NaN where that is outside the vocabulary. ids and values may both be NULL, so may lse,
+ * chosen int32 [rows], NaN where that is outside the vocabulary; it is formed from the row's maximum, so that it holds
+ * where lse is beyond fp32 (an infinity). ids and values may both be NULL, so may lse,
  * and chosen with logprob. -infinity is an ordinary smallest value; a row with NaN or +infinity gives ids -1
  * and NaN. k 1 .. 128 and at most vocab; temperature from
  * FLT_MIN to 1e38.

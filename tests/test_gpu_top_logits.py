@@ -184,3 +184,32 @@ def test_two_streams_and_graph(gpu):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out[:3], G.top_logits(x, 20)[:3]))
+
+
+def test_sums_beyond_fp32_and_gaps_beyond_it(gpu):
+    """The log-probability is a difference that fp32 holds where max / T lies below its range, and where two logits are
+    further apart than its range while T brings them together."""
+    import torch
+    import ds41_gfx950 as G
+    x = torch.randn(3, 50257, device=gpu) - 100
+    best = x.max(1)
+    for T in (1e-37, 2e-38):
+        ids, values, lse, lp = G.top_logits(x, 2, temperature=T, chosen=best.indices.int())
+        assert bool((lse == -float("inf")).all()) and torch.equal(ids[:, 0], best.indices.int())
+        assert float(lp.abs().max()) <= lse_bound(50257, 0)
+        second = G.top_logits(x, 2, temperature=T, chosen=ids[:, 1].contiguous())[3].double()
+        want = (values[:, 1].double() - values[:, 0].double()) / float(np.float32(T))
+        want = torch.where(want < -torch.finfo(torch.float32).max, -float("inf"), want)
+        assert bool(((second == want) | ((second - want).abs() <= 2.0 ** -22 * want.abs())).all())
+    for n, V in ((2, 50257), (300, 40000)):  # short and long chunks
+        x = torch.full((n, V), -3e38, device=gpu)
+        x[:, 30000:30010], x[0, 17], x[1, 20000:20004] = 3e38, 1e38, 2e38
+        for T in (1e38, 5e37):
+            z = x.double() / float(np.float32(T))
+            for c in (0, 17, 30005):
+                chosen = torch.full((n,), c, dtype=torch.int32, device=gpu)
+                lse, lp = G.top_logits(x, 3, temperature=T, chosen=chosen)[2:]
+                want = z.logsumexp(1)
+                # exponents of up to 12, each a few roundings
+                assert float((lse.double() - want).abs().max()) <= lse_bound(V, 12)
+                assert float((lp.double() - (z[:, c] - want)).abs().max()) <= lse_bound(V, 12) + 24 * 2.0 ** -22
