@@ -277,3 +277,19 @@ def test_control_and_commit_in_a_graph(gpu):
         torch.cuda.synchronize()
         assert torch.equal(out_e, out_g) and torch.equal(eager[0], table[0]) and torch.equal(eager[1], table[1])
     assert int(table[0][0, 9]) == 8
+
+
+def test_totals_up_to_the_largest(gpu):
+    """total bounds the offsets; a buffer may be said to hold up to 2^31 - 1 tokens, whatever the sequences take of it."""
+    import torch
+    import ds41_gfx950 as G
+    V = 100
+    tokens, offsets = dev(np.array([5, 5, 7, 99, 1], np.int32), gpu), dev(np.array([0, 3, 5], np.int32), gpu)
+    for total in (5, (1 << 31) - 2, (1 << 31) - 1):
+        counts, seen = G.token_counts(2, V, gpu)
+        rc = G.lib().ds41_token_counts_add(counts.data_ptr(), seen.data_ptr(), 2, V, None, tokens.data_ptr(), offsets.data_ptr(), 2, total, 1,
+                                           G._stream())
+        assert rc == 0
+        want = torch.zeros(2, V, dtype=torch.int32)
+        want[0, 5], want[0, 7], want[1, 99], want[1, 1] = 2, 1, 1, 1
+        assert torch.equal(counts.cpu(), want)
