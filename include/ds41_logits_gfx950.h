@@ -107,10 +107,10 @@ int ds41_top_logits(const void *logits, int type, size_t ld, int rows, int vocab
  * Where every logit outside the set is -infinity, log q_r is -infinity, the loss +infinity if p_r > 0, and the gradient
  * outside 0. What a grammar masks of the student belongs in the renormalised form, or the teacher's rest pulls on it.
  * A row with nothing in its set has loss 0 and gradient 0 whatever its logits hold (padding). loss F32
- * [rows]; stats F32 [rows][2] = {log sum exp z, log q_r (0 when renormalised)}, which the backward call takes;
- * both 0 for such a row. A step forms its gradient from unrounded statistics; the backward call reads them rounded, so
- * that its q are off by up to 2^-24 of |log sum exp z| + |log q_r| more, and forms them again, by one workgroup a row,
- * where that sum is above 8,192. grad: grad_loss[row] (F32 [rows]) times the derivative, in the logits' type, ld_grad
+ * [rows]; stats F32 [rows][2] = {log sum exp z, log q_r (0 when renormalised) + what rounding left of the first},
+ * which the backward call takes; both 0 for such a row. The backward call's q are off by the second's own rounding, 2^-25
+ * of |log q_r|, and with a rest class by 2^-25 of |log sum exp z| too for bf16 rows and where it writes over the logits;
+ * where the two are above 8,192 together one workgroup a row forms them again. A step has none of this. grad: grad_loss[row] (F32 [rows]) times the derivative, in the logits' type, ld_grad
  * apart; grad may be logits (with ld_grad == ld) and must not overlap it otherwise. k 1 .. 128; temperature
  * 0.01 .. 100. ds41_distill_step is forward and backward in one call, for a grad_loss known beforehand.
  * workspace: ds41_distill_workspace_bytes(rows, vocab) device bytes, 256-byte aligned, which cover every call of no

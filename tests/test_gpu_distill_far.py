@@ -4,8 +4,10 @@ a logarithm (added up, a masked row's would lose the logarithm).
 
 Bounds. S as in test_gpu_distill.py, for a sum over the vocabulary. With t = |x - max| / T, an entry outside is
 weight * exp(-t) / sum: the exponent is off by at most four roundings of t (scale, product, difference), exp2 by two
-steps, the product by four more; the weight q_r - p_r by S q_r. The call that takes saved statistics reads them rounded
-to 32 bits, which counts up to 8,192: from there on it forms them again. The rest is 64-bit, and the output rounds once."""
+steps, the product by four more; the weight q_r - p_r by S q_r. Of the saved statistics, 32 bits each, the second holds
+what rounding left of the first, and is rounded itself, which counts up to 8,192: from there on the backward call forms
+them again. With a rest class, a backward call in place or of bf16 rows takes the first as it is. The rest is 64-bit, and
+the output rounds once."""
 import numpy as np
 import pytest
 
@@ -48,8 +50,8 @@ def make(gpu, seed, n, V, k, dtype, T, rest):
 
 
 def reference(x, ids, tl, tlse, gl, T, half):
-    """(loss, stats, gradient, bound of the loss, of the statistics, of a step's gradient, of a pair's). Entries left out,
-    repeated ids and rows without a set as the header defines them."""
+    """(loss, stats, gradient, bounds of the loss, of the statistics, of a step's gradient, of a pair's, of a pair's in place).
+    Entries left out, repeated ids and rows without a set as the header defines them."""
     import torch
     n, V = x.shape
     x, T = x.double(), float(np.float32(T))
@@ -76,7 +78,7 @@ def reference(x, ids, tl, tlse, gl, T, half):
         lse, logr, rest = m / T + total.log(), zero, zero
         d = q - P
         tol = q * exponent(m)
-        tol_pair = tol + q * 2.0 ** -24 * lse.abs().clamp(max=REACH)
+        tol_pair = tol_place = tol
     else:
         mi, ei, si = part(inset)
         mo, eo, so = part(~inset)
@@ -87,19 +89,24 @@ def reference(x, ids, tl, tlse, gl, T, half):
         lse = torch.where(dist > 0, mi / T + (si.log() - logi), mo / T + (so.log() - logr))
         q, weight = ei / si * logi.exp(), logr.exp() - rest
         d = torch.where(inset, q - P, weight * (eo / so))
-        saved = 2.0 ** -24 * (lse.abs() + logr.abs()).clamp(max=REACH)
         tol = torch.where(inset, q * s, (weight.abs() * exponent(mo) + logr.exp() * s + 1e-14) * (eo / so))
-        tol_pair = tol + torch.where(inset, q * 2.0 ** -24 * lse.abs().clamp(max=REACH), (weight.abs() + logr.exp()) * saved * (eo / so))
+        second, first = 2.0 ** -24 * logr.abs().clamp(max=REACH), 2.0 ** -24 * lse.abs().clamp(max=REACH)
+        tol_pair = tol + torch.where(inset, q, (weight.abs() + logr.exp()) * (eo / so)) * second
+        tol_place = tol_pair + torch.where(inset, q, logr.exp() * (eo / so)) * first
     loss = torch.where(inset & (P > 0), P * (P.log() - logq), 0.0).sum(1) + torch.where(rest > 0, rest * (rest.log() - logr), zero).squeeze(1)
     grad, stats = d * gT, torch.cat((lse, logr), 1)
     done = []
-    for t in (tol, tol_pair):
+    for t in (tol, tol_pair, tol_place):
         t = 1.05 * gT * (t + 2e-38) + 8 * 2.0 ** -24 * grad.abs()
         done.append(t + half * (grad.abs() + t) + 2e-38)
-    got = [loss, stats, grad, 2 * s + 2.0 ** -23 * loss.abs(), 2 * s + 2.0 ** -23 * stats.abs(), *done]
+    tol_s = 2 * s + 2.0 ** -23 * stats.abs()
+    tol_s[:, 1] += 2.0 ** -24 * torch.where(lse.abs() <= REACH, lse.abs(), 0.0).squeeze(1)
+    got = [loss, stats, grad, 2 * s + 2.0 ** -23 * loss.abs(), tol_s, *done]
     none = ~some.squeeze(1)
     for g in got:
         g[none] = 0
+    if half > 2.0 ** -24:
+        got[-2] = got[-1]
     return got
 
 
@@ -121,13 +128,13 @@ ROWS = {"few": {"float32": 10, "bfloat16": 10}, "chunks": {"float32": 230, "bflo
 
 def check(x, ids, tl, tlse, gl, T, dtype):
     import ds41_gfx950 as G
-    loss, stats, grad, tol_l, tol_s, tol_g, tol_p = reference(x, ids, tl, tlse, gl, T, HALF[dtype])
+    loss, stats, grad, tol_l, tol_s, tol_g, tol_p, tol_i = reference(x, ids, tl, tlse, gl, T, HALF[dtype])
     kw = dict(teacher_lse=tlse, temperature=T)
     l1, s1 = G.distill_forward(x, ids, tl, **kw)
     got = [("forward", l1, s1, None, None), ("backward", l1, s1, G.distill_backward(x, ids, tl, s1, gl, **kw), tol_p)]
     y = x.clone()
     G.distill_backward(y, ids, tl, s1, gl, grad=y, **kw)
-    got.append(("backward in place", l1, s1, y, tol_p))
+    got.append(("backward in place", l1, s1, y, tol_i))
     got.append(("step", *G.distill_step(x, ids, tl, gl, **kw), tol_g))
     y = x.clone()
     got.append(("step in place", *G.distill_step(y, ids, tl, gl, grad=y, **kw), tol_g))
