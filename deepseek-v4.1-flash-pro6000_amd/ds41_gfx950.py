@@ -483,9 +483,22 @@ def _wide(t, what, dtype, n, width):
         return None
     if t.dtype is dtype and t.is_contiguous():
         shape = t.shape
-        if shape[-1] == width and t.numel() >= n * width if len(shape) > 1 else t.numel() == n * width:
+        if len(shape) == 2:
+            if shape[1] == width and shape[0] >= n:
+                return t.data_ptr()
+        elif t.numel() == n * width if len(shape) < 2 else shape[-1] == width and t.numel() >= n * width:
             return t.data_ptr()
     raise ValueError(f"{what}: {n} contiguous rows of {width} {dtype}, not {tuple(t.shape)} {t.dtype}")
+
+
+def _matrix(t, what, dtype, n, width):
+    """The same of a matrix alone."""
+    if t is None:
+        return None
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == width and shape[0] >= n and t.dtype is dtype and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{what}: a contiguous matrix of {n} rows of {width} {dtype}, not {tuple(shape)} {t.dtype}")
 
 
 def _stream_of(stream, first, *others):
@@ -1236,11 +1249,8 @@ def token_counts(table_rows, vocab, device="cuda"):
 
 
 def _table(counts, seen, vocab):
-    rows, i32 = (counts if counts is not None else seen).shape[0], _dtypes()[2]
-    for t in (counts, seen):
-        if t is not None and len(t.shape) != 2:
-            raise ValueError(f"a token table is two matrices, not {tuple(t.shape)}")
-    return _wide(counts, "counts", i32, rows, vocab), _wide(seen, "seen", i32, rows, (vocab + 31) // 32), rows
+    i32, rows = _dtypes()[2], (counts if counts is not None else seen).shape[0]
+    return _matrix(counts, "counts", i32, rows, vocab), _matrix(seen, "seen", i32, rows, (vocab + 31) >> 5), rows
 
 
 def token_counts_clear(counts, seen, vocab, table_index=None, stream=None):
