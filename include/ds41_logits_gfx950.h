@@ -9,7 +9,8 @@
  * engine/src/hotpath/batch.inc:496,553). All buffers are caller-owned DEVICE memory; `stream` is a
  * hipStream_t passed as void*; every entry returns a hipError_t value as int, invalid arguments
  * hipErrorInvalidValue (1) before any launch. No entry allocates or synchronises, and every one may be
- * captured into a graph. vocab 1 .. 1,048,576 (as the samplers), rows and sequences 1 .. 65,535.
+ * captured into a graph. vocab 1 .. 1,048,576 (as the samplers), rows and sequences 1 .. 65,535 (ds41_logits_control: 1 .. 64
+ * rows a sequence).
  * A row stride (ld) counts elements and is at least vocab; rows need the alignment of their element only.
  */
 #ifndef DS41_LOGITS_GFX950_H
