@@ -101,7 +101,9 @@ def reference(x, ids, tl, tlse, gl, T, half):
         done.append(t + half * (grad.abs() + t) + 2e-38)
     tol_s = 2 * s + 2.0 ** -23 * stats.abs()
     tol_s[:, 1] += 2.0 ** -24 * torch.where(lse.abs() <= REACH, lse.abs(), 0.0).squeeze(1)
-    got = [loss, stats, grad, 2 * s + 2.0 ** -23 * loss.abs(), tol_s, *done]
+    # what the set leaves of 1 is off by 128 terms' 2^-53 (1.4e-14) either way, times log q_r, which a mask makes 1e38
+    tol_l = 2 * s + 2.0 ** -23 * loss.abs() + torch.where(rest > 0, 2 * 1.4e-14 * logr.abs(), zero).squeeze(1)
+    got = [loss, stats, grad, tol_l, tol_s, *done]
     none = ~some.squeeze(1)
     for g in got:
         g[none] = 0
