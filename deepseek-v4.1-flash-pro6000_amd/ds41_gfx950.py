@@ -635,7 +635,7 @@ def _saved(t, M, I):
 def ffn_forward(x, w_gate, w_up, w_down, limit=0.0, out=None, saved=None, workspace=None, stream=None):
     """(silu(x w_gate^T) * (x w_up^T)) w_down^T in bf16, x [M][H], w_gate and w_up [I][H], w_down [H][I], with the gate cut at
     limit and the up projection at both (0: neither). saved: a float32 or (less exact) bfloat16 tensor [M][2 I] for the
-    backward call."""
+    backward call. No output may lie over an input."""
     bf16 = _dtypes()[1]
     M, H, I, args = _ffn(x, w_gate, w_up, w_down)
     out, ldy = _as(out, "out", bf16, (M, H), stream, x)
@@ -648,7 +648,8 @@ def ffn_forward(x, w_gate, w_up, w_down, limit=0.0, out=None, saved=None, worksp
 def ffn_backward(x, w_gate, w_up, w_down, saved, grad_out, limit=0.0, grad_x=None, grad_gate=None, grad_up=None, grad_down=None,
                  grad_dtype=None, accumulate=False, workspace=None, stream=None):
     """(grad_x, grad_gate, grad_up, grad_down) of ffn_forward from what it saved; the weights' gradients of grad_dtype (that of those
-    given, else bfloat16). False for one of the four: it is not formed. accumulate: the weights' are added to what is there."""
+    given, else bfloat16). False for one of the four: it is not formed. accumulate: the weights' are added to what is there. No
+    gradient may lie over an input (grad_x over grad_out, say): the ones after it still read that."""
     f32, bf16, _ = _dtypes()
     M, H, I, args = _ffn(x, w_gate, w_up, w_down)
     if grad_out.shape != (M, H):

@@ -1,0 +1,140 @@
+"""Whether two lists of rows share a byte, compiled for the host and compared with every byte marked, and the calls that
+refuse outputs over their inputs: every check runs on the host before any launch, so the addresses are never read."""
+import os
+import subprocess
+
+import pytest
+
+import ds41_gfx950 as G
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PROGRAM = r"""
+#include <cstdio>
+#include <vector>
+#include "memory_rows.hpp"
+using namespace ds41g;
+static bool marked(const MemoryRows &a, const MemoryRows &b) {
+  std::vector<char> m(4096);
+  for (size_t r = 0; r < a.rows; ++r)
+    for (size_t i = 0; i < a.bytes; ++i) m[a.at + r * a.stride + i] = 1;
+  for (size_t r = 0; r < b.rows; ++r)
+    for (size_t i = 0; i < b.bytes; ++i)
+      if (m[b.at + r * b.stride + i]) return true;
+  return false;
+}
+int main() {
+  long seen = 0, meet = 0;
+  for (size_t ra : {1, 2, 5}) for (size_t wa : {1, 3, 4}) for (size_t sa : {4, 6, 9})
+    for (size_t rb : {1, 2, 3, 7}) for (size_t wb : {1, 2, 4}) for (size_t sb : {4, 6, 11})
+      for (size_t at = 1; at < 120; ++at) {
+        const MemoryRows a{40, ra, wa, sa}, b{at, rb, wb, sb};
+        const bool want = marked(a, b);
+        if (memory_meets(a, b) != want || memory_meets(b, a) != want) {
+          std::printf("%zu %zu %zu, %zu: %zu %zu %zu\n", ra, wa, sa, at, rb, wb, sb);
+          return 1;
+        }
+        ++seen;
+        meet += want;
+      }
+  if (memory_meets(memory_block(nullptr, 8), memory_block(nullptr, 8))) return 2;
+  const MemoryRows out[] = {memory_block((void *)100, 8), memory_block((void *)108, 8)}, in[] = {memory_block((void *)116, 8)};
+  const MemoryRows over[] = {memory_block((void *)100, 9), memory_block((void *)108, 8)}, read[] = {memory_block((void *)115, 8)};
+  if (memory_collides(out, in) || !memory_collides(over, in) || !memory_collides(out, read)) return 3;
+  std::printf("%ld %ld\n", seen, meet);
+}
+"""
+
+
+def test_rows_that_share_a_byte(tmp_path):
+    src, exe = tmp_path / "rows.cpp", tmp_path / "rows"
+    src.write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(ROOT, "deepseek-v4.1-flash-pro6000_amd", "csrc"),
+                    str(src), "-o", str(exe)], check=True, timeout=120)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
+    seen, meet = map(int, r.stdout.split())
+    assert seen > 100000 and seen // 10 < meet < seen
+
+
+INVALID = 1
+
+
+def at(i):
+    """Addresses far apart."""
+    return (i + 1) << 32
+
+
+def call(name, args, **change):
+    return getattr(G.lib(), "ds41_" + name)(*dict(args, **change).values())
+
+
+def accepted(rc):
+    """The checks let the call pass: without a GPU its launch then fails with another error."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses must not be launched with")
+    assert rc not in (0, INVALID)
+
+
+M, H, I = 5, 64, 40
+FFN = dict(x=at(0), ldx=H, w_gate=at(1), w_up=at(2), w_down=at(3), limit=10.0)
+FORWARD = dict(FFN, y=at(4), ldy=H, saved=at(5), saved_type=0, M=M, H=H, I=I, ws=at(6), ws_bytes=1 << 30, stream=None)
+BACKWARD = dict(FFN, saved=at(5), saved_type=0, grad_y=at(4), ld_grad_y=H, grad_x=at(7), ld_grad_x=H, grad_gate=at(8), grad_up=at(9),
+                grad_down=at(10), grad_type=1, accumulate=0, M=M, H=H, I=I, ws=at(6), ws_bytes=1 << 30, stream=None)
+
+
+@pytest.mark.parametrize("change", [
+    dict(y=at(0)), dict(y=at(0) + 2 * H * (M - 1)), dict(y=at(1)), dict(y=at(2) + 2 * I * H - 16), dict(y=at(3)), dict(y=at(5)), dict(y=at(6) + 256),
+    dict(saved=at(0)), dict(saved=at(1)), dict(saved=at(3) + 16), dict(saved=at(4) + 16), dict(saved=at(6)),
+    dict(saved=at(0) - 4 * 2 * I * M + 16), dict(ws=at(0)), dict(ws=at(1)), dict(ws=at(3)),
+    dict(x=at(0), ldx=160, y=at(0) + 2 * 56, ldy=160)])  # rows of one buffer, eight columns shared
+def test_ffn_forward_refuses_outputs_over_inputs(change):
+    accepted(call("ffn_forward", FORWARD))
+    assert call("ffn_forward", FORWARD, **change) == INVALID
+
+
+@pytest.mark.parametrize("change", [
+    dict(grad_x=at(4)),                                          # over the gradient that the down projection's still reads
+    dict(grad_x=at(0)),                                          # over the rows that the gate's and the up projection's still read
+    dict(grad_x=at(1)), dict(grad_x=at(2)), dict(grad_x=at(3)), dict(grad_x=at(5) + 16), dict(grad_x=at(6)), dict(grad_x=at(8)),
+    dict(grad_gate=at(0)), dict(grad_gate=at(1)), dict(grad_gate=at(4)), dict(grad_gate=at(9)), dict(grad_up=at(2)), dict(grad_up=at(0) + 16),
+    dict(grad_up=at(10)), dict(grad_down=at(3)), dict(grad_down=at(4)), dict(grad_down=at(5)), dict(grad_down=at(7) + 16),
+    dict(grad_gate=at(9) - 4 * I * H + 16, grad_type=0),         # fp32 gradients reach twice as far
+    dict(ws=at(0)), dict(ws=at(5)), dict(ws=at(10)),
+    dict(ldx=160, grad_x=at(0) + 2 * 56, ld_grad_x=160)])
+def test_ffn_backward_refuses_outputs_over_inputs(change):
+    accepted(call("ffn_backward", BACKWARD))
+    assert call("ffn_backward", BACKWARD, **change) == INVALID
+
+
+def test_ffn_takes_columns_of_one_buffer():
+    accepted(call("ffn_forward", FORWARD, ldx=2 * H, y=at(0) + 2 * H, ldy=2 * H))
+    accepted(call("ffn_forward", FORWARD, ldx=2 * H + 8, y=at(0) + 2 * H, ldy=2 * H + 8))
+    accepted(call("ffn_forward", FORWARD, w_up=at(1)))  # inputs may be the same
+    accepted(call("ffn_forward", FORWARD, saved=None))
+    accepted(call("ffn_backward", BACKWARD, ldx=2 * H, grad_x=at(0) + 2 * H, ld_grad_x=2 * H))
+    accepted(call("ffn_backward", BACKWARD, grad_gate=at(9) - 2 * I * H))
+    accepted(call("ffn_backward", BACKWARD, grad_gate=at(9) - 4 * I * H, grad_type=0))
+    accepted(call("ffn_backward", BACKWARD, grad_x=None, grad_up=None))
+    accepted(call("ffn_backward", BACKWARD, grad_gate=None, grad_up=None, grad_down=None))
+    # a workspace that reaches over another tensor behind what the call needs
+    accepted(call("ffn_forward", FORWARD, ws=at(4) - (G.ffn_workspace_bytes(M, H, I) + 255) // 256 * 256))
+
+
+# The refusals of the block's other arguments, each by itself: distinct addresses, so that nothing else refuses them.
+BOTH = [dict(x=None), dict(w_gate=None), dict(w_up=None), dict(w_down=None), dict(ldx=63), dict(ldx=56), dict(ldx=68), dict(x=at(0) + 8),
+        dict(w_gate=at(1) + 8), dict(w_up=at(2) + 2), dict(w_down=at(3) + 4), dict(limit=-1.0), dict(limit=float("nan")), dict(limit=float("inf")),
+        dict(M=0), dict(M=(1 << 20) + 1), dict(H=0), dict(H=60), dict(I=0), dict(I=44), dict(I=65544), dict(ws=None), dict(ws=at(6) + 16),
+        dict(ws_bytes=256), dict(saved=at(5) + 8), dict(saved_type=2), dict(saved_type=-1)]
+
+
+@pytest.mark.parametrize("change", BOTH + [dict(y=None), dict(ldy=56), dict(ldy=65), dict(y=at(4) + 8)])
+def test_ffn_forward_refusals_alone(change):
+    assert call("ffn_forward", FORWARD, **change) == INVALID
+
+
+@pytest.mark.parametrize("change", BOTH + [
+    dict(saved=None), dict(grad_y=None), dict(ld_grad_y=63), dict(ld_grad_x=56), dict(grad_x=at(7) + 8), dict(grad_gate=at(8) + 8), dict(grad_up=at(9) + 4),
+    dict(grad_down=at(10) + 2), dict(grad_type=2), dict(grad_type=-1)])
+def test_ffn_backward_refusals_alone(change):
+    assert call("ffn_backward", BACKWARD, **change) == INVALID
