@@ -57,7 +57,8 @@ int ds41_quantize_mxfp8(const void *x_bf16, uint8_t *q, uint8_t *scales, int row
  * max |x| <= 6 * 2^e, and q [rows][cols / 2] the e2m1 codes nearest to x / 2^e, ties to the even code, even columns in the low
  * half of a byte: the layout of the expert tensors above. values_bf16 (nullable) [rows][cols]: what the codes stand for,
  * exactly. A group with an infinity or NaN gets scale 255, codes 0 and values NaN; what would round to 2^128 gets the next
- * code below. q is 4-byte aligned; no output may overlap x or another output. */
+ * code below. q is 4-byte aligned; outputs that share a byte
+ * with x or with another output are refused, as an x between elements is. */
 int ds41_quantize_mxfp4(const void *x, int type, size_t ldx, uint8_t *q, uint8_t *scales, void *values_bf16,
                         int rows, int cols, void *stream);
 /* grouped_mxfp4 / _native / _parallel / _native_parallel / _native_tiled

@@ -68,12 +68,13 @@ def call(name, args, **change):
     return getattr(G.lib(), "ds41_" + name)(*dict(args, **change).values())
 
 
-def accepted(rc):
-    """The checks let the call pass: without a GPU its launch then fails with another error."""
+def accepted(name, args, **change):
+    """The checks let the call pass: without a GPU its launch then fails with another error. With one it is not made, since its
+    addresses are of nothing."""
     import torch
     if torch.cuda.is_available():
-        pytest.skip("the addresses must not be launched with")
-    assert rc not in (0, INVALID)
+        pytest.skip("no call with these addresses where there is a GPU")
+    assert call(name, args, **change) not in (0, INVALID)
 
 
 M, H, I = 5, 64, 40
@@ -89,7 +90,7 @@ BACKWARD = dict(FFN, saved=at(5), saved_type=0, grad_y=at(4), ld_grad_y=H, grad_
     dict(saved=at(0) - 4 * 2 * I * M + 16), dict(ws=at(0)), dict(ws=at(1)), dict(ws=at(3)),
     dict(x=at(0), ldx=160, y=at(0) + 2 * 56, ldy=160)])  # rows of one buffer, eight columns shared
 def test_ffn_forward_refuses_outputs_over_inputs(change):
-    accepted(call("ffn_forward", FORWARD))
+    accepted("ffn_forward", FORWARD)
     assert call("ffn_forward", FORWARD, **change) == INVALID
 
 
@@ -103,22 +104,22 @@ def test_ffn_forward_refuses_outputs_over_inputs(change):
     dict(ws=at(0)), dict(ws=at(5)), dict(ws=at(10)),
     dict(ldx=160, grad_x=at(0) + 2 * 56, ld_grad_x=160)])
 def test_ffn_backward_refuses_outputs_over_inputs(change):
-    accepted(call("ffn_backward", BACKWARD))
+    accepted("ffn_backward", BACKWARD)
     assert call("ffn_backward", BACKWARD, **change) == INVALID
 
 
 def test_ffn_takes_columns_of_one_buffer():
-    accepted(call("ffn_forward", FORWARD, ldx=2 * H, y=at(0) + 2 * H, ldy=2 * H))
-    accepted(call("ffn_forward", FORWARD, ldx=2 * H + 8, y=at(0) + 2 * H, ldy=2 * H + 8))
-    accepted(call("ffn_forward", FORWARD, w_up=at(1)))  # inputs may be the same
-    accepted(call("ffn_forward", FORWARD, saved=None))
-    accepted(call("ffn_backward", BACKWARD, ldx=2 * H, grad_x=at(0) + 2 * H, ld_grad_x=2 * H))
-    accepted(call("ffn_backward", BACKWARD, grad_gate=at(9) - 2 * I * H))
-    accepted(call("ffn_backward", BACKWARD, grad_gate=at(9) - 4 * I * H, grad_type=0))
-    accepted(call("ffn_backward", BACKWARD, grad_x=None, grad_up=None))
-    accepted(call("ffn_backward", BACKWARD, grad_gate=None, grad_up=None, grad_down=None))
+    accepted("ffn_forward", FORWARD, ldx=2 * H, y=at(0) + 2 * H, ldy=2 * H)
+    accepted("ffn_forward", FORWARD, ldx=2 * H + 8, y=at(0) + 2 * H, ldy=2 * H + 8)
+    accepted("ffn_forward", FORWARD, w_up=at(1))  # inputs may be the same
+    accepted("ffn_forward", FORWARD, saved=None)
+    accepted("ffn_backward", BACKWARD, ldx=2 * H, grad_x=at(0) + 2 * H, ld_grad_x=2 * H)
+    accepted("ffn_backward", BACKWARD, grad_gate=at(9) - 2 * I * H)
+    accepted("ffn_backward", BACKWARD, grad_gate=at(9) - 4 * I * H, grad_type=0)
+    accepted("ffn_backward", BACKWARD, grad_x=None, grad_up=None)
+    accepted("ffn_backward", BACKWARD, grad_gate=None, grad_up=None, grad_down=None)
     # a workspace that reaches over another tensor behind what the call needs
-    accepted(call("ffn_forward", FORWARD, ws=at(4) - (G.ffn_workspace_bytes(M, H, I) + 255) // 256 * 256))
+    accepted("ffn_forward", FORWARD, ws=at(4) - (G.ffn_workspace_bytes(M, H, I) + 255) // 256 * 256)
 
 
 # The refusals of the block's other arguments, each by itself: distinct addresses, so that nothing else refuses them.
@@ -138,3 +139,30 @@ def test_ffn_forward_refusals_alone(change):
     dict(grad_down=at(10) + 2), dict(grad_type=2), dict(grad_type=-1)])
 def test_ffn_backward_refusals_alone(change):
     assert call("ffn_backward", BACKWARD, **change) == INVALID
+
+
+QUANT = dict(x=at(0), type=0, ldx=64, q=at(1), scales=at(2), values=at(3), rows=3, cols=64, stream=None)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=at(0)), dict(q=at(0) + 4 * 191), dict(scales=at(0) + 767), dict(values=at(0), type=1), dict(values=at(0) - 382, type=1), dict(q=at(3)),
+    dict(q=at(3) + 380), dict(scales=at(1) + 95), dict(scales=at(1) - 5), dict(values=at(2)), dict(ldx=80, q=at(0) + 4 * 80),
+    dict(x=at(0) + 2), dict(x=at(0) + 1, type=1)])  # an address between elements
+def test_quantize_refuses_outputs_over_its_rows_and_rows_between_elements(change):
+    accepted("quantize_mxfp4", QUANT)
+    assert call("quantize_mxfp4", QUANT, **change) == INVALID
+
+
+def test_quantize_takes_outputs_beside_its_rows():
+    accepted("quantize_mxfp4", QUANT, q=at(0) + 4 * 192)
+    accepted("quantize_mxfp4", QUANT, scales=at(0) - 6)
+    accepted("quantize_mxfp4", QUANT, scales=at(1) + 96, values=None)
+    accepted("quantize_mxfp4", QUANT, rows=1, ldx=128, q=at(0) + 256)
+    accepted("quantize_mxfp4", QUANT, rows=1, cols=32, ldx=40, x=at(0) + 4, scales=at(0) + 132)
+    accepted("quantize_mxfp4", QUANT, x=at(0) + 2, type=1)
+
+
+@pytest.mark.parametrize("change", [dict(x=None), dict(q=None), dict(scales=None), dict(type=2), dict(type=-1), dict(ldx=63), dict(rows=0),
+                                    dict(rows=-1), dict(cols=0), dict(cols=48), dict(q=at(1) + 2), dict(values=at(3) + 1)])
+def test_quantize_refusals_alone(change):
+    assert call("quantize_mxfp4", QUANT, **change) == INVALID
