@@ -1550,7 +1550,8 @@ def _policy_out(logits, loss, logprob, stats, workspace, stream):
 
 def policy_forward(logits, tokens, old_logprob, advantage, ref_logprob=None, kl_coef=0.0, clip_low=0.2, clip_high=0.2, temperature=1.0,
                    loss=None, logprob=None, stats=None, workspace=None, stream=None):
-    """(loss [rows], logprob [rows], stats [rows][3]) of fp32 or bf16 rows: the clipped policy loss of each row's token."""
+    """(loss [rows], logprob [rows], stats [rows][3]) of fp32 or bf16 rows: the clipped policy loss of each row's token. No
+    output may lie over an input (logprob over old_logprob, say)."""
     args = _policy(logits, tokens, old_logprob, advantage, ref_logprob, kl_coef, clip_low, clip_high, temperature)
     out, outs, ws = _policy_out(logits, loss, logprob, stats, workspace, stream)
     check(lib().ds41_policy_forward(*args, *outs, ws.data_ptr(), ws.nbytes,
@@ -1572,7 +1573,8 @@ def policy_backward(logits, tokens, old_logprob, advantage, stats, grad_loss, re
 
 def policy_step(logits, tokens, old_logprob, advantage, grad_loss, ref_logprob=None, kl_coef=0.0, clip_low=0.2, clip_high=0.2,
                 temperature=1.0, loss=None, logprob=None, stats=None, grad=None, workspace=None, stream=None):
-    """(loss, logprob, stats, grad): policy_forward and policy_backward in one call."""
+    """(loss, logprob, stats, grad): policy_forward and policy_backward in one call; of the outputs only grad may lie over an
+    input, the logits."""
     args = _policy(logits, tokens, old_logprob, advantage, ref_logprob, kl_coef, clip_low, clip_high, temperature)
     grad, ld_grad = _grad(logits, grad, stream)
     out, outs, ws = _policy_out(logits, loss, logprob, stats, workspace, stream)

@@ -146,7 +146,8 @@ int ds41_distill_step(const void *logits, int type, size_t ld, int rows, int voc
  * chosen one; a row with NaN or +infinity gives NaN.
  * loss, logprob F32 [rows]; stats F32 [rows][3] (the largest of the other logits, the sum of their exponentials from there, the
  * chosen token's logit), which the backward call takes: it forms the step's gradient. grad: grad_loss[row] (F32 [rows]) times the
- * derivative, in the logits' type, ld_grad apart; grad may be logits (with ld_grad == ld) and must not overlap it otherwise.
+ * derivative, in the logits' type, ld_grad apart; grad may be logits (with ld_grad == ld). Outputs (the workspace among them) that
+ * otherwise share a byte with an input or with another output are refused.
  * clip_low 0 .. 1, clip_high and kl_coef finite and not negative, temperature 0.01 .. 100. ds41_policy_step is forward and
  * backward in one call.
  * workspace: ds41_policy_workspace_bytes(rows, vocab) device bytes, 256-byte aligned, which cover every call of no

@@ -166,3 +166,59 @@ def test_quantize_takes_outputs_beside_its_rows():
                                     dict(rows=-1), dict(cols=0), dict(cols=48), dict(q=at(1) + 2), dict(values=at(3) + 1)])
 def test_quantize_refusals_alone(change):
     assert call("quantize_mxfp4", QUANT, **change) == INVALID
+
+
+N, V = 6, 1000
+POLICY = dict(logits=at(0), type=0, ld=V, rows=N, vocab=V, tokens=at(1), old=at(2), advantage=at(3), ref=at(4), kl=0.1, low=0.2, high=0.3, temperature=1.0)
+P_FORWARD = dict(POLICY, loss=at(6), logprob=at(7), stats=at(8), ws=at(9), ws_bytes=1 << 20, stream=None)
+P_BACKWARD = dict(POLICY, stats=at(8), grad_loss=at(5), grad=at(10), ld_grad=V, stream=None)
+P_STEP = dict(POLICY, grad_loss=at(5), loss=at(6), logprob=at(7), stats=at(8), grad=at(10), ld_grad=V, ws=at(9), ws_bytes=1 << 20, stream=None)
+
+
+@pytest.mark.parametrize("change", [
+    # a row's workgroups read these after the first of them has written its loss and log-probability
+    dict(logprob=at(2)), dict(loss=at(3)), dict(loss=at(2) + 4), dict(logprob=at(4) + 20), dict(stats=at(2)), dict(stats=at(1) - 4),
+    dict(loss=at(7)), dict(loss=at(8) + 68), dict(logprob=at(8)), dict(ws=at(0)), dict(ws=at(2)), dict(ws=at(6)), dict(loss=at(9) + 4),
+    dict(loss=at(0)), dict(logprob=at(0) + 4 * 5999), dict(stats=at(1))])
+def test_policy_refuses_outputs_over_inputs(change):
+    accepted("policy_forward", P_FORWARD)
+    accepted("policy_step", P_STEP)
+    assert call("policy_forward", P_FORWARD, **change) == INVALID
+    assert call("policy_step", P_STEP, **change) == INVALID
+
+
+@pytest.mark.parametrize("change", [
+    dict(grad=at(0) + 4), dict(grad=at(0) - 4), dict(grad=at(0), ld=V + 1), dict(grad=at(0) + 4 * 5999), dict(grad=at(2)), dict(grad=at(5)), dict(grad=at(4)),
+    dict(grad=at(1)), dict(grad=at(8)), dict(ld=2 * V, grad=at(0) + 4 * (V - 1), ld_grad=2 * V), dict(ld=V + 8, grad=at(0) + 4 * V, ld_grad=V + 8)])
+def test_policy_refuses_gradients_over_inputs(change):
+    accepted("policy_backward", P_BACKWARD)
+    assert call("policy_backward", P_BACKWARD, **change) == INVALID
+    assert call("policy_step", P_STEP, **change) == INVALID
+
+
+def test_policy_takes_gradients_in_place_and_beside():
+    for name, args in (("policy_backward", P_BACKWARD), ("policy_step", P_STEP)):
+        accepted(name, args, grad=at(0))
+        accepted(name, args, type=1, grad=at(0))
+        accepted(name, args, ld=2 * V, grad=at(0) + 4 * V, ld_grad=2 * V)
+        accepted(name, args, ref=None, kl=0.0)
+    accepted("policy_step", P_STEP, ref=at(6), kl=0.0)  # not read
+    accepted("policy_forward", P_FORWARD, old=at(4))
+
+
+@pytest.mark.parametrize("change", [
+    dict(logits=None), dict(type=2), dict(type=-1), dict(ld=999), dict(rows=0), dict(rows=65536), dict(vocab=0), dict(vocab=(1 << 20) + 1, ld=1 << 21),
+    dict(tokens=None), dict(old=None), dict(advantage=None), dict(ref=None), dict(kl=-0.1), dict(kl=float("nan")), dict(kl=float("inf")), dict(low=-0.1),
+    dict(low=1.1), dict(low=float("nan")), dict(high=-0.1), dict(high=float("inf")), dict(temperature=0.0), dict(temperature=1000.0), dict(stats=None)])
+def test_policy_refusals_alone(change):
+    for name, args in (("policy_forward", P_FORWARD), ("policy_backward", P_BACKWARD), ("policy_step", P_STEP)):
+        assert call(name, args, **change) == INVALID, name
+
+
+def test_policy_refusals_of_outputs_alone():
+    for change in (dict(loss=None), dict(logprob=None), dict(ws=None), dict(ws=at(9) + 8), dict(ws_bytes=1)):
+        assert call("policy_forward", P_FORWARD, **change) == INVALID
+        assert call("policy_step", P_STEP, **change) == INVALID
+    for change in (dict(grad=None), dict(grad_loss=None), dict(ld_grad=999), dict(grad=at(0), ld_grad=1001)):
+        assert call("policy_backward", P_BACKWARD, **change) == INVALID
+        assert call("policy_step", P_STEP, **change) == INVALID
