@@ -222,3 +222,45 @@ def test_policy_refusals_of_outputs_alone():
     for change in (dict(grad=None), dict(grad_loss=None), dict(ld_grad=999), dict(grad=at(0), ld_grad=1001)):
         assert call("policy_backward", P_BACKWARD, **change) == INVALID
         assert call("policy_step", P_STEP, **change) == INVALID
+
+
+def grads(*entries):
+    a = (G.GradDesc * len(entries))(*(G.GradDesc(*e) for e in entries))
+    a.n = len(entries)
+    return a
+
+
+def grad_call(name, entries, *rest):
+    import ctypes
+    a = grads(*entries)
+    return getattr(G.lib(), "ds41_" + name)(ctypes.addressof(a), a.n, *rest, None)
+
+
+LIST = [(at(0), None, 100, 0, 0), (at(1), at(2), 51, 1, 0), (None, None, 0, 0, 0)]
+
+
+def grad_accepted(name, *rest):
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("no call with these addresses where there is a GPU")
+    assert grad_call(name, LIST, *rest) not in (0, INVALID)
+
+
+@pytest.mark.parametrize("norm", [at(0), at(0) + 396, at(2) + 100])
+def test_clip_refuses_a_norm_inside_its_outputs(norm):
+    """A workgroup would scale it while others still read it."""
+    grad_accepted("grad_clip", at(5), 1.0)
+    grad_accepted("grad_clip", at(0) + 400, 1.0)
+    grad_accepted("grad_clip", at(1), 1.0)  # read, not written
+    assert grad_call("grad_clip", LIST, norm, 1.0) == INVALID
+
+
+@pytest.mark.parametrize("norm,square,ws", [
+    (at(0), None, at(6)), (at(5), at(0) + 392, at(6)), (at(1) + 100, None, at(6)), (at(5), None, at(0)), (at(5), None, at(1)),
+    (at(5), None, at(0) - 2048 * 8), (at(6) + 8, None, at(6)), (at(5), at(6), at(6)), (at(5), at(5), at(6)), (at(5) + 4, at(5), at(6))])
+def test_grad_norm_refuses_outputs_over_gradients_or_each_other(norm, square, ws):
+    grad_accepted("grad_norm", at(5), at(5) + 8, at(6), 1 << 20)
+    grad_accepted("grad_norm", at(0) + 400, at(5), at(6), 1 << 20)
+    grad_accepted("grad_norm", at(2), None, at(6), 1 << 20)  # clipping's outputs are not this call's
+    change = 0 if ws != at(0) - 2048 * 8 else 256  # reaches over the first gradient by 256 bytes
+    assert grad_call("grad_norm", LIST, norm, square, ws + change, 1 << 20) == INVALID
