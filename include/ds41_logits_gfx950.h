@@ -174,7 +174,8 @@ int ds41_policy_step(const void *logits, int type, size_t ld, int rows, int voca
  * ds41_grad_norm: norm F32 [1] = sqrt(sum of all squares), square_sum F64 [1] (nullable) the sum itself, for adding over
  * processes. Squares are formed and added in fp64 in a fixed order: the same bits every call for the same list.
  * ds41_grad_clip: out = grad * min(1, max_norm / (*norm + 1e-6)) with norm read on the device; out NULL or grad: in place,
- * where nothing is written if the factor is 1. The product is rounded once. A norm of infinity gives a factor of 0 (so
+ * where nothing is written if the factor is 1. Factor and product are formed in fp64, rounded to fp32 and, of bf16 gradients,
+ * from there to bf16. A norm of infinity gives a factor of 0 (so
  * infinities become NaN), a norm of NaN gives NaN everywhere. Outputs that overlap each other, a gradient that is not
  * their own, or norm are refused, as ds41_grad_norm's are over a gradient or each other. max_norm finite and not negative.
  * workspace: ds41_grad_workspace_bytes(n) device bytes, 256-byte aligned; calls that share one must be ordered. */
