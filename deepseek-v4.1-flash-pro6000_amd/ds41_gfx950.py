@@ -193,6 +193,7 @@ _SIGNATURES = {
     "Q:i": "grad_workspace_bytes",
     "i:pipppQp": "grad_norm",
     "i:pipfp": "grad_clip",
+    "i:pifpppQp": "grad_norm_clip",
     "i:piQpppiip": "quantize_mxfp4",
     "i:pQpppfpQpiiiipQp": "ffn_forward",
     "i:pQpppfpipQpQpppiiiiipQp": "ffn_backward",
@@ -1633,35 +1634,38 @@ def _grads_stream(stream, every, norm, *others):
     return _stream_of(stream, every[0], norm, *others)
 
 
-def _norm_of(grads, norm, square_sum, words, every, workspace, stream):
+def _norm_of(grads, norm, square_sum, every, workspace, stream):
+    """(norm, the addresses of it and of square_sum, a workspace and its size, the stream) of a call that forms a norm."""
     import torch
     f32, n = _dtypes()[0], len(grads)
     norm = _new(stream, grads[0], (1,), f32) if norm is None else norm
     ws = _workspace(workspace, lambda: lib().ds41_grad_workspace_bytes(n), grads[0], stream)
     s = _grads_stream(stream, every, norm, square_sum, ws)
-    check(lib().ds41_grad_norm(words.buffer_info()[0], n, _flat(norm, "norm", f32, 1), _flat(square_sum, "square_sum", torch.float64, 1),
-                               ws.data_ptr(), ws.nbytes, s), "ds41_grad_norm")
-    return norm, s
+    return norm, (_flat(norm, "norm", f32, 1), _flat(square_sum, "square_sum", torch.float64, 1), ws.data_ptr(), ws.nbytes, s)
 
 
 def grad_norm(grads, norm=None, square_sum=None, workspace=None, stream=None):
     """The norm (float32 [1]) of a list of gradients; square_sum: a float64 tensor [1] for the sum of the squares."""
     grads = list(grads)
     words, every = _grads(grads, None)
-    return _norm_of(grads, norm, square_sum, words, every, workspace, stream)[0]
+    norm, rest = _norm_of(grads, norm, square_sum, every, workspace, stream)
+    check(lib().ds41_grad_norm(words.buffer_info()[0], len(grads), *rest), "ds41_grad_norm")
+    return norm
 
 
-def grad_clip(grads, max_norm, out=None, norm=None, known=False, workspace=None, stream=None):
-    """Clips a list of gradients to max_norm, in place or into out; returns their norm before. known: norm is given (that of
-    all processes' gradients, say) and is not formed."""
+def grad_clip(grads, max_norm, out=None, norm=None, known=False, workspace=None, stream=None, square_sum=None):
+    """Clips a list of gradients to max_norm, in place or into out; returns their norm before. The factor is of the norm before its
+    rounding to float32; square_sum as in grad_norm. known: norm is given (that of all processes' gradients, say) and is not formed."""
     grads = list(grads)
     words, every = _grads(grads, None if out is None else list(out))
     if known:
         if norm is None:
             raise ValueError("known: a norm")
-        norm_p, s = _flat(norm, "norm", _dtypes()[0], 1), _grads_stream(stream, every, norm)
-    else:
-        norm, s = _norm_of(grads, norm, None, words, every, workspace, stream)
-        norm_p = norm.data_ptr()
-    check(lib().ds41_grad_clip(words.buffer_info()[0], len(grads), norm_p, max_norm, s), "ds41_grad_clip")
+        if square_sum is not None:
+            raise ValueError("known: no sum is formed")
+        check(lib().ds41_grad_clip(words.buffer_info()[0], len(grads), _flat(norm, "norm", _dtypes()[0], 1), max_norm,
+                                   _grads_stream(stream, every, norm)), "ds41_grad_clip")
+        return norm
+    norm, rest = _norm_of(grads, norm, square_sum, every, workspace, stream)
+    check(lib().ds41_grad_norm_clip(words.buffer_info()[0], len(grads), max_norm, *rest), "ds41_grad_norm_clip")
     return norm

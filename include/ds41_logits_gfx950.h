@@ -175,9 +175,11 @@ int ds41_policy_step(const void *logits, int type, size_t ld, int rows, int voca
  * processes. Squares are formed and added in fp64 in a fixed order: the same bits every call for the same list.
  * ds41_grad_clip: out = grad * min(1, max_norm / (*norm + 1e-6)) with norm read on the device; out NULL or grad: in place,
  * where nothing is written if the factor is 1. Factor and product are formed in fp64, rounded to fp32 and, of bf16 gradients,
- * from there to bf16. A norm of infinity gives a factor of 0 (so
- * infinities become NaN), a norm of NaN gives NaN everywhere. Outputs that overlap each other, a gradient that is not
- * their own, or norm are refused, as ds41_grad_norm's are over a gradient or each other. max_norm finite and not negative.
+ * from there to bf16. A norm of infinity gives a factor of 0 (so infinities become NaN), a norm of NaN gives NaN everywhere.
+ * ds41_grad_norm_clip: both in one call, with the factor of the norm before its rounding to fp32: infinite only where a
+ * gradient is, not where finite gradients have a norm beyond fp32 (then *norm alone is infinity).
+ * Outputs that overlap each other, a gradient that is not their own, norm, square_sum or the workspace are refused, as
+ * ds41_grad_norm's are over a gradient or each other. max_norm finite and not negative.
  * workspace: ds41_grad_workspace_bytes(n) device bytes, 256-byte aligned; calls that share one must be ordered. */
 enum { DS41_GRAD_MAX = 65535 };
 typedef struct {
@@ -190,6 +192,8 @@ size_t ds41_grad_workspace_bytes(int n);
 int ds41_grad_norm(const ds41_grad *grads, int n, float *norm, double *square_sum, void *workspace,
                    size_t workspace_bytes, void *stream);
 int ds41_grad_clip(const ds41_grad *grads, int n, const float *norm, float max_norm, void *stream);
+int ds41_grad_norm_clip(const ds41_grad *grads, int n, float max_norm, float *norm, double *square_sum,
+                        void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -264,3 +264,23 @@ def test_grad_norm_refuses_outputs_over_gradients_or_each_other(norm, square, ws
     grad_accepted("grad_norm", at(2), None, at(6), 1 << 20)  # clipping's outputs are not this call's
     change = 0 if ws != at(0) - 2048 * 8 else 256  # reaches over the first gradient by 256 bytes
     assert grad_call("grad_norm", LIST, norm, square, ws + change, 1 << 20) == INVALID
+
+
+@pytest.mark.parametrize("entries,limit,norm,square,ws", [
+    (LIST, 1.0, at(0), None, at(6)), (LIST, 1.0, at(2) + 100, None, at(6)), (LIST, 1.0, at(5), at(2), at(6)), (LIST, 1.0, at(5), None, at(2)),
+    (LIST, 1.0, at(5), None, at(2) - 2048 * 8), (LIST, 1.0, at(1), None, at(6)), (LIST, 1.0, at(6), None, at(6)), (LIST, 1.0, at(5), at(5), at(6)),
+    (LIST, -1.0, at(5), None, at(6)), (LIST, float("nan"), at(5), None, at(6)), (LIST, float("inf"), at(5), None, at(6)), (LIST, 1.0, None, None, at(6)),
+    (LIST, 1.0, at(5), None, None), (LIST, 1.0, at(5), None, at(6) + 8), (LIST + LIST[:1], 1.0, at(5), None, at(6)),
+    ([(at(0), at(1), 100, 0, 0), (at(1), at(0), 100, 0, 0)], 1.0, at(5), None, at(6)), ([(at(0), None, 100, 2, 0)], 1.0, at(5), None, at(6))])
+def test_norm_and_clip_refusals(entries, limit, norm, square, ws):
+    grad_accepted("grad_norm_clip", 1.0, at(5), at(5) + 8, at(6), 1 << 20)
+    grad_accepted("grad_norm_clip", 1.0, at(5), None, at(6), G.lib().ds41_grad_workspace_bytes(len(LIST)))
+    assert grad_call("grad_norm_clip", entries, limit, norm, square, ws, 1 << 20) == INVALID
+    assert grad_call("grad_norm_clip", entries, 1.0, at(5), None, at(6), G.lib().ds41_grad_workspace_bytes(len(entries)) - 1) == INVALID
+
+
+def test_binding_refuses_a_sum_of_a_known_norm():
+    import torch
+    one = torch.zeros(1)
+    with pytest.raises(ValueError, match="no sum"):
+        G.grad_clip([torch.zeros(3)], 1.0, norm=one, known=True, square_sum=one.double())
