@@ -147,6 +147,7 @@ _SIGNATURES = {
     "i:ppiiiiip": "grouped_mxfp4_prefill",
     "i:piiiiip": "moe_prefill_tiles moe_prefill_plan_counts",
     "i:iip": "expert_slab_layout",
+    "i:iiip": "ffn_plan",
     "i:ppiii": "expert_slab_tile_host",
     "i:pppippppp": "verify_stack_step",
     "i:pippipppp": "verify_stack_layer",
@@ -600,6 +601,16 @@ def dense_bf16(x, w, bias=None, residual=None, act="none", out=None, out_dtype=N
 @functools.lru_cache(4096)
 def ffn_workspace_bytes(M, H, I):
     return lib().ds41_ffn_workspace_bytes(M, H, I)
+
+
+FFN_PRODUCTS = ("gate_up", "y", "dh", "grad_x", "grad_gate_up", "grad_one", "grad_down")
+
+
+def ffn_plan(M, H, I):
+    """{product: (side of a tile, tiles, how many are formed whole, parts of the sum in each of the others)} of a block's calls."""
+    p = (ctypes.c_int32 * 28)()
+    check(lib().ds41_ffn_plan(M, H, I, ctypes.addressof(p)), "ds41_ffn_plan")
+    return {name: tuple(p[4 * i:4 * i + 4]) for i, name in enumerate(FFN_PRODUCTS)}
 
 
 def _exact(t, what, dtype, shape):

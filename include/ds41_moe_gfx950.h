@@ -422,6 +422,10 @@ int ds41_dense_bf16(const void *x_bf16, size_t ldx, const void *w_bf16, size_t l
  * workspace: ds41_ffn_workspace_bytes(M, H, I) device bytes, 256-byte aligned, which cover forward and backward calls of no more
  * rows with the same H and I; calls that share one must be ordered. */
 size_t ds41_ffn_workspace_bytes(int M, int H, int I);
+/* The tiles that the block's products are formed in, for tests and measurements: plan (a host array) [7][4] = side of a tile, tiles,
+ * how many of them are formed whole, parts of the sum in each of the others. In order: g and u; y; dh; grad_x; grad_gate and
+ * grad_up together; one of those two alone; grad_down. Four times 0 for what takes no tiles (the forward call's of at most 32 rows). */
+int ds41_ffn_plan(int M, int H, int I, int32_t *plan);
 int ds41_ffn_forward(const void *x, size_t ldx, const void *w_gate, const void *w_up, const void *w_down,
                      float limit, void *y, size_t ldy, void *saved, int saved_type, int M, int H, int I, void *workspace,
                      size_t workspace_bytes, void *stream);
