@@ -414,7 +414,7 @@ int ds41_dense_bf16(const void *x_bf16, size_t ldx, const void *w_bf16, size_t l
  *   grad_x = dg w_gate + du w_up (bf16 [M][H], ld_grad_x),
  *   grad_gate = dg^T x, grad_up = du^T x ([I][H]), grad_down = grad_y^T h ([H][I]), of type grad_type (DS41_TYPE_F32 or _BF16),
  *   contiguous; each of the four may be NULL and is then not formed. accumulate != 0: the three weights' gradients are added to what
- *   is there (rounded once). dg, du and h are rounded to bf16 for the products, whose sums are fp32.
+ *   is there, in fp32, and the result is rounded to their type. dg, du and h are rounded to bf16 for the products, whose sums are fp32.
  * M 1 .. 1,048,576, H and I multiples of 8, 8 .. 65,536; pointers 16-byte aligned and strides multiples of 8 (of one row any). Outputs (the
  * workspace among them) that share an element with an input or with another output are refused; rows beside each other in one
  * buffer are not. The same call gives the same bits; the order of a sum follows from the sizes and from
