@@ -39,3 +39,29 @@ def test_sums_of_even_rows(gpu, dtype, n, V):
         assert off.max() <= BOUND, (off.max() * 2.0 ** 24, np.sqrt((off ** 2).mean()) * 2.0 ** 24)
         # log p, of size 11: the sum's error and half a step of its own
         assert ((logprob.double() - lp).abs() <= BOUND + lp.abs() * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("n,V", [(30, 129280), (400, 129280), (600, 50257)])
+def test_a_rows_factor_is_rounded_once(gpu, n, V):
+    """The gradient of a row's other tokens is a factor times their exponentials. Logits N(16, 0.1^2), whose exponents are taken from an
+    offset of 23 or so that is itself rounded. What an entry's own roundings do averages out over a row (its gradient's half step
+    too: 2^-24 / sqrt(V)), so the mean of its entries over the formula's, at the maximum and sum that the call left, is off by the
+    factor's one rounding, 2^-24, and by 1.5e-8 of the temperature's as above."""
+    import torch
+    g = torch.Generator(device=gpu).manual_seed(n + V)
+    x = torch.empty((n, V), device=gpu).normal_(16, 0.1, generator=g)
+    tok = torch.randint(0, V, (n,), device=gpu, generator=g).int()
+    at = tok.long().unsqueeze(1)
+    one = torch.ones(n, device=gpu)
+    old = torch.log_softmax(x.double(), 1).gather(1, at).squeeze(1).float()
+    loss, logprob, stats, grad = G.policy_step(x, tok, old, one, one)
+    back = G.policy_backward(x, tok, old, one, stats, one)
+    m, s, xa = (stats[:, i].double() for i in range(3))
+    assert torch.equal(xa, x.double().gather(1, at).squeeze(1))
+    d = xa - m - torch.log(s)
+    slope = -torch.exp(-torch.log1p(torch.exp(-d)) - old.double())
+    want = -(slope / (1 + torch.exp(d)) / s).unsqueeze(1) * torch.exp(x.double() - m.unsqueeze(1))
+    want.scatter_(1, at, float("nan"))
+    for t in (grad, back):
+        off = ((t.double() / want).nanmean(1) - 1).abs().cpu().numpy()
+        assert off.max() <= BOUND, off.max() * 2.0 ** 24
